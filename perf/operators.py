@@ -196,7 +196,7 @@ def _own(s):
     out = {"h": h, "y": y}
     if train:
         out["dx"], out["dresidual"], out["dweight"], out["dbias"] = ops.dropout_add_layer_norm_backward(
-            h, s["dy"], s["dh"], mean, rstd, weight, x_dtype=x.dtype, **rng)
+            h, s["dy"], s["dh"], mean, rstd, weight, **rng)
     return out
 
 
