@@ -344,6 +344,53 @@ int m3d_bn_act_backward(const float* d_x, const float* d_dy, const float* d_y, i
 size_t m3d_bn_stats_static_max_bytes(void);
 int m3d_bn_stats_static(const float* d_x, int64_t n, int c, float* d_mean, float* d_var, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Layer norm, dropout, and the residual add that joins them, on [n, c] activations of type M3D_TYPE_F32 / _BF16 / _F16
+ * (0 <= n < 2^32 rows, 1 <= c <= 16384 channels for the norms; any channel count and row stride ld* >= c in elements,
+ * any address a multiple of the element size).  They are nn.LayerNorm and nn.Dropout of the reference's transformer
+ * decoder on point features (mosaic3d/src/models/networks/opensegment3d).  Outputs are contiguous; weight and bias
+ * (`wtype`: f32 or the activations' type) may be NULL (1 and 0).  Sums are f32, each output is rounded once.
+ *
+ *   m3d_layer_norm_fwd:       y = (x - mean) * rstd * weight + bias;  d_mean[n], d_rstd[n] (f32) = mean and
+ *                             1 / sqrt(biased variance + eps) of the row, for the backward pass
+ *   m3d_layer_norm_backward:  with hat = (x - mean) * rstd, g = dy * weight:  dx = rstd * (g - mean(g) - hat * mean(g * hat));
+ *                             dweight = sum_r dy * hat and dbias = sum_r dy (`wtype`; either or both NULL = not wanted)
+ *                             in a fixed order.  Workspace (with dweight or dbias):
+ *                             m3d_layer_norm_workspace_bytes(n, c, type), 16-byte aligned
+ *   m3d_dropout:              y = kept ? x / (1 - p) : 0.  Its backward pass is the same call on the gradient.
+ *   m3d_dropout_add_layer_norm_fwd:  h = residual + dropout(x), rounded to `stream_type` (`type` or f32), and
+ *                             y = layer norm of h as it was rounded.  d_h = NULL: h is not written
+ *   m3d_dropout_add_layer_norm_backward:  t = dh + layer norm's input gradient at h (d_dh = NULL: 0);
+ *                             dresidual = t (`stream_type`), dx = dropout(t) (`type`), either may be NULL
+ *
+ * Dropout masks: value (row, channel) is kept where a 32-bit word is at least round(p * 2^32).  The word is number
+ * channel % 4 of the Philox 4x32 block (7 rounds) with counter (channel / 4, row, offset low, offset high) and key
+ * (seed low, seed high).  The mask depends on nothing else and is never stored; calls with different offsets are
+ * independent.  d_state != NULL: seed = d_state[0] and d_state[1] is added to `offset`, read on the device, so that a
+ * captured graph draws new masks on every replay; m3d_dropout_next copies the state's two words to d_used and adds
+ * `step` to the second. */
+#define M3D_TYPE_F32 0
+#define M3D_TYPE_BF16 1
+#define M3D_TYPE_F16 2
+size_t m3d_layer_norm_workspace_bytes(int64_t n, int c, int type);
+int m3d_layer_norm_fwd(const void* d_x, int64_t ldx, int type, int64_t n, int c, const void* d_weight, const void* d_bias,
+                       int wtype, float eps, void* d_y, float* d_mean, float* d_rstd, void* stream);
+int m3d_layer_norm_backward(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, int type, int64_t n, int c,
+                            const float* d_mean, const float* d_rstd, const void* d_weight, int wtype, void* d_dx,
+                            void* d_dweight, void* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
+int m3d_dropout(const void* d_x, int64_t ldx, int type, int64_t n, int c, double p, uint64_t seed, uint64_t offset,
+                const int64_t* d_state, void* d_y, void* stream);
+int m3d_dropout_next(int64_t* d_state, int64_t step, int64_t* d_used, void* stream);
+int m3d_dropout_add_layer_norm_fwd(const void* d_x, int64_t ldx, int type, const void* d_residual, int64_t ldr,
+                                   int stream_type, int64_t n, int c, const void* d_weight, const void* d_bias, int wtype,
+                                   float eps, double p, uint64_t seed, uint64_t offset, const int64_t* d_state, void* d_h,
+                                   void* d_y, float* d_mean, float* d_rstd, void* stream);
+int m3d_dropout_add_layer_norm_backward(const void* d_h, int64_t ldh, int stream_type, const void* d_dy, int64_t lddy,
+                                        int type, const void* d_dh, int64_t lddh, int64_t n, int c, const float* d_mean,
+                                        const float* d_rstd, const void* d_weight, int wtype, double p, uint64_t seed,
+                                        uint64_t offset, const int64_t* d_state, void* d_dx, void* d_dresidual,
+                                        void* d_dweight, void* d_dbias, void* d_ws, size_t ws_bytes, void* stream);
+
 /* `terms` of the split-format entry points is 1, 2, 3 (bf16 terms) or M3D_FMT_F16_PAIR: [rows + 1][C/32][2][32] f16,
  * term 0 = f16(x), term 1 = f16((x - term 0) * 2^11).
  * m3d_f16_status: every kernel that writes the pair format sets a per-device status word when a value lies beyond

@@ -19,6 +19,8 @@ Pinning status
   pinned against outputs of the reference's own CLIPAlignmentEval.predict (on the features of the reference's own
   forward pass) and CaptionLoss.loss / extract_text_features with their gradients (tests/golden/reference_loss.npz,
   produced by tests/golden/make_golden_loss.py from /root/reference).
+* layer norm, dropout and their residual add (oracle/layer_norm.py): float64 formulas; the dropout generator is checked
+  against its authors' published known answers (tests/test_layers.py).
 * sparse-conv kernel maps and convolution arithmetic: the reference delegates these to the
   un-vendored third-party wheel ``spconv-cu120`` (version unpinned in
   /root/reference/mosaic3d/requirements.txt:41), which is not installed anywhere and has no
@@ -34,4 +36,5 @@ from .sparse_conv import (subm_conv, strided_conv, inverse_conv, conv1x1, dense_
 from .head import head_logits, head_predict
 from . import preprocess
 from . import caption_loss
+from . import layer_norm
 from .spunet import spunet_forward, fold_pdnorm, make_spunet_params, SPUNET34C

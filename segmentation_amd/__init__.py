@@ -6,5 +6,5 @@ The kernels live in libm3d_hip.so next to this file; operators raise if it is mi
 no CPU fallback."""
 from . import _lib  # noqa: F401
 
-__all__ = ["ops", "sparse", "spunet", "engine", "compat", "scenes"]
+__all__ = ["ops", "sparse", "layers", "spunet", "engine", "compat", "scenes"]
 __version__ = "0.1.0"

@@ -58,6 +58,18 @@ SIGNATURES = {
     "m3d_bn_stats_static_max_bytes": (_sz, []),
     "m3d_bn_stats_static": (_int, [_vp, _i64, _int, _vp, _vp, _vp]),
     "m3d_bn_backward_reduce": (_int, [_vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _sz, _vp]),
+    "m3d_layer_norm_workspace_bytes": (_sz, [_i64, _int, _int]),
+    "m3d_layer_norm_fwd": (_int, [_vp, _i64, _int, _i64, _int, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp]),
+    "m3d_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp,
+                                       _sz, _vp]),
+    "m3d_dropout": (_int, [_vp, _i64, _int, _i64, _int, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp, _vp]),
+    "m3d_dropout_next": (_int, [_vp, _i64, _vp, _vp]),
+    "m3d_dropout_add_layer_norm_fwd": (_int, [_vp, _i64, _int, _vp, _i64, _int, _i64, _int, _vp, _vp, _int, _f32,
+                                              ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp, _vp, _vp, _vp,
+                                              _vp]),
+    "m3d_dropout_add_layer_norm_backward": (_int, [_vp, _i64, _int, _vp, _i64, _int, _vp, _i64, _i64, _int, _vp, _vp, _vp,
+                                                   _int, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp, _vp,
+                                                   _vp, _vp, _vp, _sz, _vp]),
     "m3d_sf32_bytes": (_sz, [_i64, _int, _int]),
     "m3d_split_f32": (_int, [_vp, _i64, _int, _int, _vp, _vp]),
     "m3d_conv_packed_weight_bytes": (_sz, [_int, _int, _int, _int]),

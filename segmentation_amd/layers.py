@@ -1,0 +1,156 @@
+"""Layer norm, dropout and the residual add that joins them, as differentiable functions and modules over the kernels of
+ops.layer_norm_fwd, ops.dropout and ops.dropout_add_layer_norm_fwd: what a transformer block on point features is made
+of around its matrix products (nn.LayerNorm and nn.Dropout in mosaic3d/src/models/networks/opensegment3d).
+
+Activations [..., c] in float32, bfloat16 or float16, weight and bias in the same type or float32.  First derivatives
+only.  Dropout masks are functions of (seed, offset, row, channel) and are recomputed in the backward pass."""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dweight, dbias = ops.layer_norm_backward(x, dy, mean, rstd, weight, ctx.needs_input_grad[1],
+                                                     ctx.needs_input_grad[2])
+        return dx, dweight, dbias, None
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, state):
+        ctx.drop = (p, seed, offset, state)
+        return ops.dropout(x, *ctx.drop)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return ops.dropout(dy, *ctx.drop), None, None, None, None
+
+
+class _DropoutAddLayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, p, seed, offset, state):
+        y, h, mean, rstd = ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state)
+        ctx.save_for_backward(h, weight, mean, rstd)
+        ctx.drop = dict(p=p, seed=seed, offset=offset, state=state)
+        ctx.x_dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight, mean, rstd = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        if dy is None:   # only h was used
+            if dh is None:
+                return (None,) * 9
+            dy = torch.zeros(h.shape, dtype=ctx.x_dtype, device=h.device)
+        grads = ops.dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight, **ctx.drop, want_dx=want[0],
+                                                    want_dresidual=want[1], want_dweight=want[2], want_dbias=want[3])
+        return (*grads, None, None, None, None, None)
+
+
+def _taped(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last axis (ops.layer_norm_fwd), differentiable in x, weight and bias."""
+    if not _taped(x, weight, bias):
+        return ops.layer_norm_fwd(x, weight, bias, eps)[0]
+    return _LayerNormFn.apply(x, weight, bias, eps)
+
+
+def dropout(x, p=0.5, training=True, seed=0, offset=0, state=None):
+    """Dropout (ops.dropout), differentiable in x; x itself outside training or with p = 0.  Calls that shall draw
+    masks of their own differ in seed, offset or state (ops.dropout_next)."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability {p} is not in [0, 1]")
+    if not training or p == 0.0:
+        return x
+    if not _taped(x):
+        return ops.dropout(x, p, seed, offset, state)
+    return _DropoutFn.apply(x, p, seed, offset, state)
+
+
+def dropout_add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, training=True, seed=0, offset=0,
+                           state=None):
+    """(y, h) with h = residual + dropout(x) and y = layer norm of h (ops.dropout_add_layer_norm_fwd), differentiable in
+    x, residual, weight and bias through both outputs; no dropout outside training.  The residual stream is of x's type or
+    float32."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability {p} is not in [0, 1]")
+    if not training or p == 0.0:
+        p, seed, offset, state = 0.0, 0, 0, None
+    if not _taped(x, residual, weight, bias):
+        return ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state)[:2]
+    return _DropoutAddLayerNormFn.apply(x, residual, weight, bias, eps, p, seed, offset, state)
+
+
+class LayerNorm(nn.Module):
+    """nn.LayerNorm over the last axis: same parameter names, so its state dict loads unchanged."""
+
+    def __init__(self, num_features, eps=1e-5, affine=True):
+        super().__init__()
+        if not 1 <= num_features <= ops.LAYER_NORM_MAX_CHANNELS:
+            raise ValueError(f"LayerNorm: 1 to {ops.LAYER_NORM_MAX_CHANNELS} features, got {num_features}")
+        self.num_features, self.eps, self.affine = int(num_features), float(eps), affine
+        self.weight = nn.Parameter(torch.ones(num_features)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_features)) if affine else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return f"{self.num_features}, eps={self.eps}, affine={self.affine}"
+
+
+class Dropout(nn.Module):
+    """Dropout whose generator state is a buffer `rng` (seed, offset) on the module's device: it is saved with the
+    model, and a captured graph draws a new mask on every replay.  Without a seed one is drawn from torch's generator;
+    ranks that shall draw different masks are given different seeds."""
+
+    def __init__(self, p=0.5, seed=None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability {p} is not in [0, 1]")
+        self.p = float(p)
+        if seed is None:
+            seed = int(torch.randint(0, 2 ** 62, ()))
+        self.register_buffer("rng", ops.dropout_state(seed, "cpu"))
+
+    def draw(self):
+        """The (seed, offset) of one call, or None where nothing is dropped."""
+        return ops.dropout_next(self.rng) if self.training and self.p > 0.0 else None
+
+    def forward(self, x):
+        return dropout(x, self.p, self.training, state=self.draw())
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+
+class DropoutAddLayerNorm(nn.Module):
+    """(x, residual) -> (y, h): h = residual + dropout(x), y = layer norm of h."""
+
+    def __init__(self, num_features, p=0.0, eps=1e-5, affine=True, seed=None):
+        super().__init__()
+        self.norm = LayerNorm(num_features, eps, affine)
+        self.drop = Dropout(p, seed)
+
+    def forward(self, x, residual):
+        return dropout_add_layer_norm(x, residual, self.norm.weight, self.norm.bias, self.norm.eps, self.drop.p,
+                                      self.training, state=self.drop.draw())

@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops, sparse
+from . import layers, ops, sparse
 
 CONDITIONS = ("ScanNet", "ARKitScenes", "Matterport3D", "Structured3D", "ScanNetPP")
 SPUNET34C = dict(in_channels=3, out_channels=768, base_channels=32, context_channels=256,
@@ -33,13 +33,20 @@ class PDBatchNorm(nn.Module):
         super().__init__()
         self.conditions = tuple(conditions)
         self.decouple, self.adaptive, self.affine = decouple, adaptive, affine
-        mk = lambda: nn.BatchNorm1d(num_features, eps=eps, momentum=momentum, affine=affine)
+        mk = lambda: self._make_norm(num_features, eps, momentum, affine)
         if decouple:
             self.bns = nn.ModuleList([mk() for _ in self.conditions])
         else:
             self.bn = mk()
         if adaptive:
             self.modulation = nn.Sequential(nn.SiLU(), nn.Linear(context_channels, 2 * num_features, bias=True))
+
+    @staticmethod
+    def _make_norm(num_features, eps, momentum, affine):
+        return nn.BatchNorm1d(num_features, eps=eps, momentum=momentum, affine=affine)
+
+    def _norm_with(self, norm, feat, weight, bias, residual, relu):
+        return _batch_norm_with(norm, feat, weight, bias, residual, relu)
 
     def pick(self, condition):
         if not self.decouple:
@@ -54,10 +61,10 @@ class PDBatchNorm(nn.Module):
         library's kernels."""
         bn = self.pick(condition)
         if not self.adaptive:
-            return _batch_norm_with(bn, feat, bn.weight, bn.bias, residual, relu)
+            return self._norm_with(bn, feat, bn.weight, bn.bias, residual, relu)
         pre = self.__dict__.pop("_affine", None)  # set for one call by SpUNet.forward (all norms in one product)
         if pre is not None and feat.dim() == 2:
-            return _batch_norm_with(bn, feat, pre[0], pre[1], residual, relu)
+            return self._norm_with(bn, feat, pre[0], pre[1], residual, relu)
         assert context is not None
         shift, scale = self.modulation(context).chunk(2, dim=1)
         if bn.affine and shift.shape[0] == 1 and feat.dim() == 2:
@@ -65,8 +72,41 @@ class PDBatchNorm(nn.Module):
             # norm with weight gamma*(1+scale) and bias beta*(1+scale)+shift, so the two [N, C] elementwise passes
             # (and the three of their backward) become operations on [C] vectors.
             gain = 1.0 + scale[0]
-            return _batch_norm_with(bn, feat, bn.weight * gain, bn.bias * gain + shift[0], residual, relu)
+            return self._norm_with(bn, feat, bn.weight * gain, bn.bias * gain + shift[0], residual, relu)
+        return self._modulated(bn, feat, scale, shift, residual, relu)
+
+    def _modulated(self, bn, feat, scale, shift, residual, relu):
         return _finish(bn(feat) * (1.0 + scale) + shift, residual, relu)
+
+
+class PDLayerNorm(PDBatchNorm):
+    """PDBatchNorm with layer norms (the norms that Point Prompt Training pairs with transformer blocks): the same
+    per-dataset affine pairs under the same parameter names, the same context modulation, no running statistics.  A
+    residual is added in FRONT of the norm, as in a post-norm block: y = relu?(layer norm(residual + dropout(x))), one
+    pass each way (layers.dropout_add_layer_norm).  `eps` and `momentum` of the batch norms are not used."""
+
+    def __init__(self, num_features, context_channels=256, conditions=CONDITIONS, decouple=True, adaptive=False,
+                 affine=True, dropout=0.0):
+        super().__init__(num_features, context_channels, conditions=conditions, decouple=decouple, adaptive=adaptive,
+                         affine=affine)
+        self.drop = layers.Dropout(dropout) if dropout > 0.0 else None
+
+    @staticmethod
+    def _make_norm(num_features, eps, momentum, affine):
+        return layers.LayerNorm(num_features, affine=affine)
+
+    def _norm_with(self, norm, feat, weight, bias, residual, relu):
+        if residual is None:
+            y = layers.layer_norm(feat, weight, bias, norm.eps)
+        else:
+            state = self.drop.draw() if self.drop is not None else None
+            p = self.drop.p if state is not None else 0.0
+            y, _ = layers.dropout_add_layer_norm(feat, residual, weight, bias, norm.eps, p, state=state)
+        return F.relu(y) if relu else y
+
+    def _modulated(self, norm, feat, scale, shift, residual, relu):
+        y = self._norm_with(norm, feat, norm.weight, norm.bias, residual, False) * (1.0 + scale) + shift
+        return F.relu(y) if relu else y
 
 
 def _finish(y, residual, relu):
@@ -180,8 +220,14 @@ class SpUNet(nn.Module):
     def __init__(self, in_channels=3, out_channels=768, num_classes=0, base_channels=32, context_channels=256,
                  channels=SPUNET34C["channels"], layers=SPUNET34C["layers"], conditions=CONDITIONS,
                  zero_init=True, norm_decouple=True, norm_adaptive=True, norm_affine=True,
-                 hash_method="fnv", pooling_method="mean", pooling_seed=0):
+                 hash_method="fnv", pooling_method="mean", pooling_seed=0, norm="batch", dropout=0.0):
+        """norm="layer": PDLayerNorm in place of PDBatchNorm, with `dropout` on the residual branch of every block while
+        training (runs and trains here; the fused engine takes batch norms only)."""
         super().__init__()
+        if norm not in ("batch", "layer"):
+            raise ValueError(f"unknown norm {norm!r} (batch or layer)")
+        if not 0.0 <= dropout < 1.0 or (dropout and norm != "layer"):
+            raise ValueError('dropout is in [0, 1) and needs norm="layer"')
         # voxelizer options of spconv_unet_v1m1_base.SpUNetBase (v1m1:177-178, :335-339); v1m3 always runs the defaults
         self.hash_method, self.pooling_method, self.pooling_seed = hash_method, pooling_method, pooling_seed
         # True: forward stops in front of `final` and returns its input as sparse_conv_feat (for callers that fold
@@ -193,26 +239,28 @@ class SpUNet(nn.Module):
         self.num_stages = len(layers) // 2
         self.conditions = tuple(conditions)
         self.zero_init = zero_init
-        norm = lambda c: PDBatchNorm(c, context_channels, 1e-3, 0.01, self.conditions, norm_decouple,
-                                     norm_adaptive, norm_affine)
+        make_norm = (lambda c: PDLayerNorm(c, context_channels, self.conditions, norm_decouple, norm_adaptive, norm_affine,
+                                           dropout)) if norm == "layer" else \
+                    (lambda c: PDBatchNorm(c, context_channels, 1e-3, 0.01, self.conditions, norm_decouple, norm_adaptive,
+                                           norm_affine))
         ch = self.channels
         self.conv_input = ConvNormAct(
             sparse.SubMConv3d(in_channels, base_channels, kernel_size=3, padding=1, bias=False, indice_key="stem"),
-            norm(base_channels))
+            make_norm(base_channels))
         self.down, self.up, self.enc, self.dec = nn.ModuleList(), nn.ModuleList(), nn.ModuleList(), nn.ModuleList()
         enc_c, dec_c = base_channels, ch[-1]
         for s in range(self.num_stages):
             self.down.append(ConvNormAct(
                 sparse.SparseConv3d(enc_c, ch[s], kernel_size=2, stride=2, bias=False, indice_key=f"spconv{s + 1}"),
-                norm(ch[s])))
+                make_norm(ch[s])))
             self.enc.append(sparse.SparseSequential(OrderedDict(
-                (f"block{i}", BasicBlock(ch[s], ch[s], norm, f"subm{s + 1}")) for i in range(layers[s]))))
+                (f"block{i}", BasicBlock(ch[s], ch[s], make_norm, f"subm{s + 1}")) for i in range(layers[s]))))
             self.up.append(ConvNormAct(
                 sparse.SparseInverseConv3d(ch[len(ch) - s - 2], dec_c, kernel_size=2, bias=False,
                                            indice_key=f"spconv{s + 1}"),
-                norm(dec_c)))
+                make_norm(dec_c)))
             self.dec.append(sparse.SparseSequential(OrderedDict(
-                (f"block{i}", BasicBlock(dec_c + enc_c if i == 0 else dec_c, dec_c, norm, f"subm{s}"))
+                (f"block{i}", BasicBlock(dec_c + enc_c if i == 0 else dec_c, dec_c, make_norm, f"subm{s}"))
                 for i in range(layers[len(ch) - s - 1]))))
             enc_c, dec_c = ch[s], ch[len(ch) - s - 2]
         final_out = num_classes if num_classes > 0 else out_channels
