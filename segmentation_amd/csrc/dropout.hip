@@ -24,7 +24,10 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
     const uint32_t t = base + u * kDropThreads;
     row[u] = (__umulhi(magic, t) + t) >> shift;
     col[u] = (int)(t - row[u] * per_row) * V;
-    in[u].load(x + (row0 + row[u]) * ldx + col[u], t < total ? c - col[u] : 0);
+    const T* p = x + (row0 + row[u]) * ldx + col[u];
+    const int left = t < total ? c - col[u] : 0;
+    if (left >= V) in[u].load(p);
+    else in[u].load_some(p, 0, left);
   }
 #pragma unroll
   for (int u = 0; u < kDropPieces; ++u) {
@@ -35,7 +38,10 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
     if (d.on) drop<V>(v, col[u], (uint32_t)(row0 + row[u]), key, d.last, d.scale);
 #pragma unroll
     for (int i = 0; i < V; ++i) in[u].set(i, v[i]);
-    in[u].store(y + (row0 + row[u]) * c + col[u], t < total ? c - col[u] : 0);
+    T* p = y + (row0 + row[u]) * c + col[u];
+    const int left = t < total ? c - col[u] : 0;
+    if (left >= V) in[u].store(p);
+    else in[u].store_some(p, 0, left);
   }
 }
 

@@ -68,146 +68,223 @@ struct RowSum {
   }
 };
 
-template <typename TX, typename TR, int K, bool ADD, int THREADS>
+// A lane's pieces k = 0 .. K - 1 are lane + k * g: the same for every row, and whole but for the last.  Addresses are a
+// uniform 64-bit base per tile (scalar registers) and a 32-bit byte offset per lane.
+template <int K, int V, bool RAGGED>
+struct Lane {
+  int g, lane, slot, c;
+  Place last;
+  __device__ __forceinline__ Lane(const LnArgs& a, int lg) : g(1 << lg), c(a.c) {
+    lane = threadIdx.x & (g - 1);
+    slot = threadIdx.x >> lg;
+    last = place_of<V>(lane + (K - 1) * g, c);
+  }
+  __device__ __forceinline__ Place at(int k) const {
+    return k == K - 1 ? last : Place{(lane + k * g) * V, 0, V};
+  }
+  // loads of piece k: `base` = the tile's first row, `row` = this lane's row in it
+  template <typename T>
+  __device__ __forceinline__ void load(Piece<T, V>& q, int k, const T* base, int64_t ld, int row) const {
+    const Place p = at(k);
+    const uint32_t off = (uint32_t)row * (uint32_t)ld + (uint32_t)p.col;
+    if (RAGGED && p.count < V) q.load_some(base + off, 0, p.count);
+    else q.load(base + off);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(const Piece<T, V>& q, int k, T* base, int row) const {
+    const Place p = at(k);
+    const uint32_t off = (uint32_t)row * (uint32_t)c + (uint32_t)p.col;
+    if (p.skip == 0 && p.count == V) q.store(base + off);
+    else if (RAGGED && p.skip < V) q.store_some(base + off, p.skip, p.count);
+  }
+  // is position i of piece k this lane's own?
+  __device__ __forceinline__ bool own(int k, int i) const {
+    if (k < K - 1) return true;
+    return RAGGED ? i >= last.skip && i < last.count : last.skip == 0;
+  }
+  __device__ __forceinline__ void drop(float* v, int k, uint32_t row, const DropKey& key, const DropArgs& d) const {
+    const Place p = at(k);
+    if (RAGGED && p.skip > 0) {
+      if (p.skip < V) drop_unaligned<V>(v, p.col, row, key, d.last, d.scale);
+    } else {
+      m3d::drop<V>(v, p.col, row, key, d.last, d.scale);
+    }
+  }
+};
+
+template <typename TX, typename TR, int K, bool ADD, bool RAGGED, int THREADS>
 __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(LnArgs a) {
   constexpr int V = kPiece<TX>;
   __shared__ float red[2][THREADS / 64][1];
   RowSum<THREADS, 1> row_sum{red};
-  const int g = 1 << a.lg, lane = threadIdx.x & (g - 1), slot = threadIdx.x >> a.lg, rows = THREADS >> a.lg;
-  const bool ragged = a.c % V != 0;
+  const Lane<K, V, RAGGED> at(a, a.lg);
+  const int rows = THREADS >> a.lg;
   DropKey key = {};
   if (ADD && a.drop.on) key = drop_key(a.drop);
   float w[K][V], b[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int col = (lane + k * g) * V;
-    load_params<V>(a.weight, a.wtype, col, a.c - col, 1.f, w[k]);
-    load_params<V>(a.bias, a.wtype, col, a.c - col, 0.f, b[k]);
+    load_params<V>(a.weight, a.wtype, at.at(k), 1.f, w[k]);
+    load_params<V>(a.bias, a.wtype, at.at(k), 0.f, b[k]);
   }
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const int64_t row = tile * rows + slot;
-    const int c = row < a.n ? a.c : 0;  // rows behind the last one load and store nothing
+  // The next tile's pieces are requested before this tile is reduced and written.
+  Piece<TX, V> x[K];
+  Piece<TR, V> r[ADD ? K : 1];
+  auto fetch = [&](int64_t tile) {
+    const int64_t first = tile * rows;
+    const int row = a.n - first < rows && at.slot >= (int)(a.n - first) ? (int)(a.n - first) - 1 : at.slot;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      at.load(x[k], k, static_cast<const TX*>(a.in) + first * a.ld_in, a.ld_in, row);
+      if constexpr (ADD) at.load(r[k], k, static_cast<const TR*>(a.residual) + first * a.ld_res, a.ld_res, row);
+    }
+  };
+  int64_t tile = blockIdx.x;
+  if (tile < a.tiles) fetch(tile);
+  for (; tile < a.tiles; tile += gridDim.x) {
+    const int64_t first = tile * rows;
+    const bool live = at.slot < a.n - first;  // a row behind the last one is computed as a copy of it and not stored
     float v[K][V], s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * g) * V;
-      Piece<TX, V> x;
-      x.load(static_cast<const TX*>(a.in) + row * a.ld_in + col, c - col);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = x.get(i);
+      for (int i = 0; i < V; ++i) v[k][i] = x[k].get(i);
       if constexpr (ADD) {
-        Piece<TR, V> r;
-        r.load(static_cast<const TR*>(a.residual) + row * a.ld_res + col, c - col);
-        if (a.drop.on) drop<V>(v[k], col, (uint32_t)row, key, a.drop.last, a.drop.scale);
+        if (a.drop.on) at.drop(v[k], k, (uint32_t)(first + at.slot), key, a.drop);
+        Piece<TR, V> h;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          r.set(i, r.get(i) + v[k][i]);
-          v[k][i] = r.get(i);
+          h.set(i, r[k].get(i) + v[k][i]);
+          v[k][i] = h.get(i);
         }
-        if (a.h) r.store(static_cast<TR*>(a.h) + row * a.c + col, c - col);
+        if (a.h && live) at.store(h, k, static_cast<TR*>(a.h) + first * a.c, at.slot);
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += v[k][i];
+      for (int i = 0; i < V; ++i) s[0] += at.own(k, i) ? v[k][i] : 0.f;
     }
+    if (tile + gridDim.x < a.tiles) fetch(tile + gridDim.x);
     row_sum(s, a.lg);
     const float mean = s[0] * a.inv_c;
     s[0] = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int left = c - (lane + k * g) * V;
-      const float mu = left > 0 ? mean : 0.f;  // pieces behind the row's end: all zero, and so is their deviation
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[k][i] -= mu;
-        if (ragged && i >= left) v[k][i] = 0.f;
+        v[k][i] = at.own(k, i) ? v[k][i] - mean : 0.f;
         s[0] += v[k][i] * v[k][i];
       }
-    }
     row_sum(s, a.lg);
     const float rstd = 1.f / __builtin_sqrtf(s[0] * a.inv_c + a.eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * g) * V;
       Piece<TX, V> y;
 #pragma unroll
       for (int i = 0; i < V; ++i) y.set(i, v[k][i] * rstd * w[k][i] + b[k][i]);
-      y.store(static_cast<TX*>(a.y) + row * a.c + col, c - col);
+      if (live) at.store(y, k, static_cast<TX*>(a.y) + first * a.c, at.slot);
     }
-    if (lane == 0 && row < a.n) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+    if (at.lane == 0 && live) {
+      a.mean[first + at.slot] = mean;
+      a.rstd[first + at.slot] = rstd;
     }
   }
 }
 
-template <typename TX, typename TR, int K, bool ADD, int THREADS>
+template <typename TX, typename TR, int K, bool ADD, bool RAGGED, int THREADS>
 __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(LnArgs a) {
   constexpr int V = kPiece<TX>;
   __shared__ float red[2][THREADS / 64][2];
   RowSum<THREADS, 2> row_sum{red};
-  const int g = 1 << a.lg, lane = threadIdx.x & (g - 1), slot = threadIdx.x >> a.lg, rows = THREADS >> a.lg;
+  const Lane<K, V, RAGGED> at(a, a.lg);
+  const int rows = THREADS >> a.lg, c = a.c;
   DropKey key = {};
   if (ADD && a.drop.on) key = drop_key(a.drop);
-  float w[K][V], dw[K][V], db[K][V];
+  // The weight is read from LDS for every row ([V / 4][pieces][4], conflict-free): it would take K * V registers, which
+  // the pieces in flight need.
+  extern __shared__ float lds[];  // [max(slots / 2, 1)][channels up to whole pieces]: the weight, later the joins
+  const int pieces = at.g * K;
+  for (int q = threadIdx.x; q < pieces; q += THREADS) {
+    float v[V];
+    load_params<V>(a.weight, a.wtype, place_of<V>(q, c), 1.f, v);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (lane + k * g) * V;
-    load_params<V>(a.weight, a.wtype, col, a.c - col, 1.f, w[k]);
+    for (int i = 0; i < V; ++i) lds[((i >> 2) * pieces + q) * 4 + (i & 3)] = v[i];
+  }
+  __syncthreads();
+  float dw[K][V], db[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
-  }
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const int64_t row = tile * rows + slot;
-    const int c = row < a.n ? a.c : 0;
-    const float mean = row < a.n ? a.mean[row] : 0.f, rstd = row < a.n ? a.rstd[row] : 0.f;
-    Piece<TR, V> x[K], dh[K];
-    Piece<TX, V> dy[K];
-    float s[2] = {0.f, 0.f};
+  Piece<TR, V> x[K], dh[ADD ? K : 1];
+  Piece<TX, V> dy[K];
+  float mean, rstd;
+  auto fetch = [&](int64_t tile) {
+    const int64_t first = tile * rows;
+    const int row = a.n - first < rows && at.slot >= (int)(a.n - first) ? (int)(a.n - first) - 1 : at.slot;
+    mean = a.mean[first + row];
+    rstd = a.rstd[first + row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * g) * V;
-      x[k].load(static_cast<const TR*>(a.in) + row * a.ld_in + col, c - col);
-      dy[k].load(static_cast<const TX*>(a.dy) + row * a.ld_dy + col, c - col);
-      if constexpr (ADD) dh[k].load(static_cast<const TR*>(a.dh) + row * a.ld_dh + col, a.dh ? c - col : 0);
+      at.load(x[k], k, static_cast<const TR*>(a.in) + first * a.ld_in, a.ld_in, row);
+      at.load(dy[k], k, static_cast<const TX*>(a.dy) + first * a.ld_dy, a.ld_dy, row);
     }
+  };
+  int64_t tile = blockIdx.x;
+  if (tile < a.tiles) fetch(tile);
+  for (; tile < a.tiles; tile += gridDim.x) {
+    const int64_t first = tile * rows;
+    const bool live = at.slot < a.n - first;
+    if constexpr (ADD)
+      if (a.dh) {
+        const int row = live ? at.slot : (int)(a.n - first) - 1;
+#pragma unroll
+        for (int k = 0; k < K; ++k) at.load(dh[k], k, static_cast<const TR*>(a.dh) + first * a.ld_dh, a.ld_dh, row);
+      }
+    float hat[K][V], gw[K][V], s[2] = {0.f, 0.f};
+    const float scale = rstd;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {  // positions behind the row's end have dy = 0 and add nothing
-        const float hat = (x[k].get(i) - mean) * rstd, d = dy[k].get(i), gw = d * w[k][i];
-        dw[k][i] += d * hat;
+      for (int i = 0; i < V; ++i) {
+        const float w = lds[((i >> 2) * pieces + at.lane + k * at.g) * 4 + (i & 3)];
+        hat[k][i] = (x[k].get(i) - mean) * rstd;
+        // neither a row behind the last one nor another lane's channel adds to a sum
+        const float d = live && at.own(k, i) ? dy[k].get(i) : 0.f;
+        gw[k][i] = d * w;
+        dw[k][i] += d * hat[k][i];
         db[k][i] += d;
-        s[0] += gw;
-        s[1] += gw * hat;
+        s[0] += gw[k][i];
+        s[1] += gw[k][i] * hat[k][i];
       }
+    if (tile + gridDim.x < a.tiles) fetch(tile + gridDim.x);
     row_sum(s, a.lg);
     const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * g) * V;
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float hat = (x[k].get(i) - mean) * rstd, gw = dy[k].get(i) * w[k][i];
-        v[i] = (gw - m0 - hat * m1) * rstd;
-        if constexpr (ADD) v[i] += dh[k].get(i);
+        v[i] = (gw[k][i] - m0 - hat[k][i] * m1) * scale;
+        if constexpr (ADD)
+          if (a.dh) v[i] += dh[k].get(i);
       }
       if constexpr (ADD) {
         Piece<TR, V> out;
 #pragma unroll
         for (int i = 0; i < V; ++i) out.set(i, v[i]);
-        if (a.dres) out.store(static_cast<TR*>(a.dres) + row * a.c + col, c - col);
-        if (a.drop.on) drop<V>(v, col, (uint32_t)row, key, a.drop.last, a.drop.scale);
+        if (a.dres && live) at.store(out, k, static_cast<TR*>(a.dres) + first * c, at.slot);
+        if (a.drop.on) at.drop(v, k, (uint32_t)(first + at.slot), key, a.drop);
       }
       Piece<TX, V> out;
 #pragma unroll
       for (int i = 0; i < V; ++i) out.set(i, v[i]);
-      if (a.dx) out.store(static_cast<TX*>(a.dx) + row * a.c + col, c - col);
+      if (a.dx && live) at.store(out, k, static_cast<TX*>(a.dx) + first * c, at.slot);
     }
   }
   if (a.partial == nullptr) return;
-  // The groups of a workgroup that hold the same channels are joined: lanes of a wave by shuffles, waves through LDS in
-  // wave order (a group of several waves owns its channels alone within its slot).
+  // The groups of a workgroup that hold the same channels are joined: lanes of a wave by shuffles, then the upper half of
+  // the waves' sums through LDS onto the lower half until one is left (a group of several waves owns its channels
+  // alone within its slot).
+  const int g = at.g;
   for (int o = g; o < 64; o <<= 1)
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -216,125 +293,169 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(LnArgs a) {
         dw[k][i] += __shfl_xor(dw[k][i], o);
         db[k][i] += __shfl_xor(db[k][i], o);
       }
-  const int waves = g > 64 ? g >> 6 : 1, slots = (THREADS / 64) / waves;  // slots: partial sums per channel
+  const int waves = g > 64 ? g >> 6 : 1;
   const int me = (threadIdx.x >> 6) / waves;
-  extern __shared__ float join[];  // [slots - 1][c]
+  const bool mine = (int)(threadIdx.x & 63) < g;
+  const int lane = at.lane;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    float* out = a.partial + ((int64_t)blockIdx.x * 2 + q) * a.c;
-    const bool mine = (int)(threadIdx.x & 63) < g;
-    if (q) __syncthreads();
-    if (me > 0 && mine)
+    float(&sum)[K][V] = q ? db : dw;
+    for (int half = (THREADS / 64) / waves / 2; half > 0; half >>= 1) {
+      __syncthreads();
+      if (me >= half && me < 2 * half && mine)
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int col = (lane + k * g) * V + i;
-          if (col < a.c) join[(me - 1) * a.c + col] = q ? db[k][i] : dw[k][i];
-        }
-    __syncthreads();
+          for (int i = 0; i < V; ++i) lds[((me - half) * V + i) * pieces + lane + k * g] = sum[k][i];
+      __syncthreads();
+      if (me < half && mine)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[k][i] += lds[(me * V + i) * pieces + lane + k * g];
+    }
     if (me == 0 && mine)
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int col = (lane + k * g) * V;
-        Piece<float, V> sum;
+        Piece<float, V> o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float t = q ? db[k][i] : dw[k][i];
-          if (col + i < a.c)
-            for (int m = 0; m + 1 < slots; ++m) t += join[m * a.c + col + i];
-          sum.set(i, t);
-        }
-        sum.store(out + col, a.c - col);
+        for (int i = 0; i < V; ++i) o.set(i, sum[k][i]);
+        at.store(o, k, a.partial + ((int64_t)blockIdx.x * 2 + q) * c, 0);
       }
   }
 }
 
 // dweight and dbias from the partial rows, in f64 and in a fixed order: a workgroup owns 32 columns of the 2 * c, each of
-// its 32 row groups adds every 32nd partial row, and the group sums are added in group order.
+// its 32 row groups adds every 32nd partial row, eight loads in flight, and the group sums are joined by halves.
 __global__ __launch_bounds__(1024) void ln_columns_kernel(const float* __restrict__ partial, int blocks, int c, int wtype,
                                                           void* dweight, void* dbias) {
+  constexpr int kInFlight = 8;
   __shared__ double red[32][33];
   const int e = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + e;
+  const float* p = partial + (col < 2 * c ? col : 0);
   double s = 0.0;
-  if (col < 2 * c)
-    for (int r = grp; r < blocks; r += 32) s += (double)partial[(int64_t)r * 2 * c + col];
+  int r = grp;
+  for (; r + 32 * (kInFlight - 1) < blocks; r += 32 * kInFlight) {
+    float v[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) v[i] = p[(int64_t)(r + 32 * i) * 2 * c];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) s += (double)v[i];
+  }
+  for (; r < blocks; r += 32) s += (double)p[(int64_t)r * 2 * c];
   red[grp][e] = s;
-  __syncthreads();
+  for (int half = 16; half > 0; half >>= 1) {
+    __syncthreads();
+    if (grp < half) red[grp][e] += red[grp + half][e];
+  }
   if (grp == 0 && col < 2 * c) {
-    double t = 0.0;
-    for (int r = 0; r < 32; ++r) t += red[r][e];
+    const float t = (float)red[0][e];
     void* to = col < c ? dweight : dbias;
     const int at = col < c ? col : col - c;
     if (to == nullptr) return;
-    if (wtype == M3D_TYPE_F32) static_cast<float*>(to)[at] = (float)t;
-    else if (wtype == M3D_TYPE_BF16) static_cast<bf16_t*>(to)[at] = (bf16_t)(float)t;
-    else static_cast<f16_t*>(to)[at] = (f16_t)(float)t;
+    if (wtype == M3D_TYPE_F32) static_cast<float*>(to)[at] = t;
+    else if (wtype == M3D_TYPE_BF16) static_cast<bf16_t*>(to)[at] = (bf16_t)t;
+    else static_cast<f16_t*>(to)[at] = (f16_t)t;
   }
 }
 
 // ---------------------------------------------------------------- launch shapes
 constexpr int kLnMaxChannels = 16384;
+constexpr int kLnMaxStride = 1 << 20;  // elements: a tile's rows (1024 at most) stay within 32-bit offsets
 
 struct LnShape {
   int lg, k, threads;
 };
 
-// Lanes and pieces a lane for a row of `pieces` 16-byte pieces: the (lanes, K) that leave the fewest places empty.
-static LnShape ln_shape(int pieces, int k_max) {
+// Lanes and pieces a lane for a row of `pieces` 16-byte pieces: the (lanes, K) that leave the fewest places empty, the
+// larger K where two leave the same.
+static LnShape ln_shape(int c, int type) {
+  const int pieces = (int)cdiv(c, type == M3D_TYPE_F32 ? 4 : 8);
   LnShape best = {0, 0, 0};
   int waste = 0;
   for (int lg = 0; lg <= 10; ++lg) {
     const int g = 1 << lg, k = (int)cdiv(pieces, g);
-    if (k > k_max || (g < 8 && g < pieces)) continue;
+    if (k > (lg < 10 ? 3 : 4) || (g < 8 && g < pieces)) continue;
     if (best.k == 0 || g * k < waste) {
-      best = {lg, k, lg > 8 ? 1024 : 256};
+      best = {lg, k, lg > 9 ? 1024 : lg > 8 ? 512 : 256};
       waste = g * k;
     }
   }
   return best;
 }
 
-static int64_t ln_blocks(int64_t tiles) { return tiles < 2048 ? tiles : 2048; }
-static int64_t ln_bwd_blocks(int64_t tiles) { return tiles < 1024 ? tiles : 1024; }
+// Workgroups: every one walks over its tiles with the next tile's pieces in flight, so that a few waves keep the memory
+// busy, and each costs a load of weight and bias, or a partial row of column sums.
+//   forward:   as many as the chip holds at 1024 threads a CU (273080 x 96 f32: 37.4 us; with half as many on rows of
+//              8192 bf16 channels 56 against 47.6 us, with four times as many 59)
+//   backward:  512 threads a CU, or 768 where a lane has 64 bytes in flight or fewer (500000 x 32 f32: 39 against 44 us;
+//              75401 x 768 bf16, 96 bytes: 71 with 512 against 83 with 768, which no longer fit the registers at once).
+//              Rows of a group of 256 lanes take workgroups of 512, two rows at a time: half the partial rows.
+constexpr int kLnCus = 256;
+static LnShape ln_bwd_shape(int c, int type) {
+  LnShape s = ln_shape(c, type);
+  if (s.lg == 8) s.threads = 512;
+  return s;
+}
+static int64_t ln_blocks(int64_t tiles, int threads) {
+  const int64_t most = kLnCus * 1024 / threads;
+  return tiles < most ? tiles : most;
+}
+static int64_t ln_bwd_blocks(int64_t tiles, const LnShape& s, int bytes_in_flight) {
+  const int64_t most = s.threads > 256 ? kLnCus : bytes_in_flight <= 64 ? 3 * kLnCus : 2 * kLnCus;
+  return tiles < most ? tiles : most;
+}
 
-template <typename TX, typename TR, bool ADD, bool BWD, int K, int THREADS>
-static int ln_launch_k(LnArgs& a, int64_t blocks, size_t lds, hipStream_t stream) {
-  if constexpr (BWD)
-    hipLaunchKernelGGL((ln_bwd_kernel<TX, TR, K, ADD, THREADS>), dim3((unsigned)blocks), dim3(THREADS), lds, stream, a);
-  else
-    hipLaunchKernelGGL((ln_fwd_kernel<TX, TR, K, ADD, THREADS>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, a);
+template <typename TX, typename TR, bool ADD, bool BWD, int K, bool RAGGED, int THREADS>
+static int ln_launch_t(LnArgs& a, int64_t blocks, size_t lds, hipStream_t stream) {
+  const dim3 grid((unsigned)blocks), block(THREADS);
+  if constexpr (BWD) {
+    static LdsGrant grant;
+    auto kernel = ln_bwd_kernel<TX, TR, K, ADD, RAGGED, THREADS>;
+    if (lds > 60 * 1024)  // below the 64 KB that every kernel may have
+      if (int rc = grant.ensure(reinterpret_cast<const void*>(kernel), lds)) return rc;
+    hipLaunchKernelGGL(kernel, grid, block, lds, stream, a);
+  } else {
+    hipLaunchKernelGGL((ln_fwd_kernel<TX, TR, K, ADD, RAGGED, THREADS>), grid, block, 0, stream, a);
+  }
   M3D_LAUNCH_CHECK();
   return M3D_OK;
 }
 
+template <typename TX, typename TR, bool ADD, bool BWD, int K, bool RAGGED>
+static int ln_launch_k(LnArgs& a, const LnShape& s, int64_t blocks, size_t lds, hipStream_t stream) {
+  // what ln_shape reaches: one piece a lane only in rows of 8 pieces or fewer, four only in the widest f32 rows
+  if constexpr (K <= 3)
+    if (s.threads == 256) return ln_launch_t<TX, TR, ADD, BWD, K, RAGGED, 256>(a, blocks, lds, stream);
+  if constexpr (K == 2 || K == 3)
+    if (s.threads == 512) return ln_launch_t<TX, TR, ADD, BWD, K, RAGGED, 512>(a, blocks, lds, stream);
+  if constexpr (K == 2 || (K > 2 && sizeof(TX) == 4))
+    if (s.threads == 1024) return ln_launch_t<TX, TR, ADD, BWD, K, RAGGED, 1024>(a, blocks, lds, stream);
+  set_error("layer norm: no kernel for %d channels", a.c);
+  return M3D_EINVAL;
+}
+
 template <typename TX, typename TR, bool ADD, bool BWD>
 static int ln_launch(LnArgs& a, int64_t* out_blocks, hipStream_t stream) {
-  const LnShape s = ln_shape((int)cdiv(a.c, kPiece<TX>), sizeof(TX) == 2 ? 2 : 4);
+  const LnShape s = BWD ? ln_bwd_shape(a.c, TypeCode<TX>::value) : ln_shape(a.c, TypeCode<TX>::value);
   a.lg = s.lg;
   a.tiles = cdiv(a.n, s.threads >> s.lg);
-  const int64_t blocks = BWD ? ln_bwd_blocks(a.tiles) : ln_blocks(a.tiles);
+  const int in_flight = s.k * kPiece<TX> * (int)(sizeof(TX) + sizeof(TR) * (ADD ? 2 : 1));
+  const int64_t blocks = BWD ? ln_bwd_blocks(a.tiles, s, in_flight) : ln_blocks(a.tiles, s.threads);
   if (out_blocks) *out_blocks = blocks;
-  const int waves = s.lg > 6 ? 1 << (s.lg - 6) : 1;
-  const size_t lds = BWD && a.partial ? (size_t)((s.threads / 64) / waves - 1) * a.c * sizeof(float) : 0;
-#define M3D_LN_CASE(KK)                                                                                  \
-  case KK:                                                                                               \
-    return s.threads == 256 ? ln_launch_k<TX, TR, ADD, BWD, KK, 256>(a, blocks, lds, stream)              \
-                            : ln_launch_k<TX, TR, ADD, BWD, KK, 1024>(a, blocks, lds, stream);
+  const int slots = (s.threads / 64) / (s.lg > 6 ? 1 << (s.lg - 6) : 1);
+  const size_t lds = BWD ? (size_t)(slots > 2 && a.partial ? slots / 2 : 1) * (s.k << s.lg) * kPiece<TX> * sizeof(float) : 0;
+  const bool ragged = a.c % kPiece<TX> != 0;
+#define M3D_LN_CASE(KK)                                                                        \
+  case KK:                                                                                     \
+    return ragged ? ln_launch_k<TX, TR, ADD, BWD, KK, true>(a, s, blocks, lds, stream)          \
+                  : ln_launch_k<TX, TR, ADD, BWD, KK, false>(a, s, blocks, lds, stream);
   switch (s.k) {
     M3D_LN_CASE(1)
     M3D_LN_CASE(2)
-    case 3:
-      if constexpr (sizeof(TX) == 4)
-        return s.threads == 256 ? ln_launch_k<TX, TR, ADD, BWD, 3, 256>(a, blocks, lds, stream)
-                                : ln_launch_k<TX, TR, ADD, BWD, 3, 1024>(a, blocks, lds, stream);
-      break;
-    case 4:
-      if constexpr (sizeof(TX) == 4)
-        return s.threads == 256 ? ln_launch_k<TX, TR, ADD, BWD, 4, 256>(a, blocks, lds, stream)
-                                : ln_launch_k<TX, TR, ADD, BWD, 4, 1024>(a, blocks, lds, stream);
-      break;
+    M3D_LN_CASE(3)
+    M3D_LN_CASE(4)
   }
 #undef M3D_LN_CASE
   set_error("layer norm: no kernel for %d channels", a.c);
@@ -370,7 +491,8 @@ static int ln_check(const char* who, int type, int stream_type, int64_t n, int c
 }
 
 static int ld_check(const char* who, int64_t n, int c, int64_t ld) {
-  M3D_CHECK_ARG(ld >= c || n <= 1, "%s: row stride %lld is smaller than the %d channels", who, (long long)ld, c);
+  M3D_CHECK_ARG(n <= 1 || (ld >= c && ld <= kLnMaxStride),
+                "%s: row stride %lld is not between the %d channels and %d", who, (long long)ld, c, kLnMaxStride);
   return M3D_OK;
 }
 
@@ -410,8 +532,8 @@ using namespace m3d;
 
 extern "C" size_t m3d_layer_norm_workspace_bytes(int64_t n, int c, int type) {
   if (n <= 0 || c <= 0 || c > kLnMaxChannels || !type_ok(type)) return 256;
-  const LnShape s = type == M3D_TYPE_F32 ? ln_shape((int)cdiv(c, 4), 4) : ln_shape((int)cdiv(c, 8), 2);
-  return align_up((size_t)ln_bwd_blocks(cdiv(n, s.threads >> s.lg)) * 2 * c * sizeof(float));
+  const LnShape s = ln_bwd_shape(c, type);
+  return align_up((size_t)ln_bwd_blocks(cdiv(n, s.threads >> s.lg), s, 0) * 2 * c * sizeof(float));  // the most of all
 }
 
 extern "C" int m3d_layer_norm_fwd(const void* d_x, int64_t ldx, int type, int64_t n, int c, const void* d_weight,

@@ -24,50 +24,62 @@ struct Piece {
   typedef T vec __attribute__((ext_vector_type(V)));
   typedef T uvec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   vec v;
-  // `left` = channels from p to the end of the row (<= 0: none); positions behind the end are zero
-  __device__ __forceinline__ void load(const T* __restrict__ p, int left) {
-    if (left >= V) {
-      v = *reinterpret_cast<const uvec*>(p);
-    } else {
+  __device__ __forceinline__ void load(const T* __restrict__ p) { v = *reinterpret_cast<const uvec*>(p); }
+  __device__ __forceinline__ void store(T* __restrict__ p) const { *reinterpret_cast<uvec*>(p) = v; }
+  // positions [from, to) only; the others load as zero
+  __device__ __forceinline__ void load_some(const T* __restrict__ p, int from, int to) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = i < left ? p[i] : (T)0.f;
-    }
+    for (int i = 0; i < V; ++i) v[i] = i >= from && i < to ? p[i] : (T)0.f;
   }
-  __device__ __forceinline__ void store(T* __restrict__ p, int left) const {
-    if (left >= V) {
-      *reinterpret_cast<uvec*>(p) = v;
-    } else {
+  __device__ __forceinline__ void store_some(T* __restrict__ p, int from, int to) const {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < left) p[i] = v[i];
-    }
+    for (int i = 0; i < V; ++i)
+      if (i >= from && i < to) p[i] = v[i];
   }
   __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
   __device__ __forceinline__ void set(int i, float f) { v[i] = (T)f; }
 };
+
+// Where a lane's piece lies in its row of c channels: channels col .. col + V - 1, of which the first `skip` belong to
+// the lane before (the last piece of a row that is no multiple of V is moved back so that it ends with the row) or,
+// with skip = V, all do (a lane without a piece of its own).  Only a row of fewer than V channels has `count` < V.
+struct Place {
+  int col, skip, count;
+};
+
+template <int V>
+__device__ __forceinline__ Place place_of(int piece, int c) {
+  const int whole = c / V;
+  if (piece < whole) return {piece * V, 0, V};
+  if (c < V) return {0, piece == 0 ? 0 : V, c};
+  return {c - V, piece == whole ? V - c % V : V, V};  // c % V == 0: V, nothing is left for this lane
+}
 
 // channels per piece: 16 bytes of the activations' type
 template <typename T> constexpr int kPiece = 16 / (int)sizeof(T);
 
 // V parameters (weight or bias, f32 or the 16-bit types) as f32; p == nullptr: `none`
 template <int V>
-__device__ __forceinline__ void load_params(const void* p, int type, int64_t at, int left, float none, float* out) {
+__device__ __forceinline__ void load_params(const void* p, int type, const Place& at, float none, float* out) {
   if (p == nullptr) {
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = none;
   } else if (type == M3D_TYPE_F32) {
     Piece<float, V> q;
-    q.load(static_cast<const float*>(p) + at, left);
+    if (at.count == V) q.load(static_cast<const float*>(p) + at.col);
+    else q.load_some(static_cast<const float*>(p), 0, at.count);
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = q.get(i);
   } else if (type == M3D_TYPE_BF16) {
     Piece<bf16_t, V> q;
-    q.load(static_cast<const bf16_t*>(p) + at, left);
+    if (at.count == V) q.load(static_cast<const bf16_t*>(p) + at.col);
+    else q.load_some(static_cast<const bf16_t*>(p), 0, at.count);
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = q.get(i);
   } else {
     Piece<f16_t, V> q;
-    q.load(static_cast<const f16_t*>(p) + at, left);
+    if (at.count == V) q.load(static_cast<const f16_t*>(p) + at.col);
+    else q.load_some(static_cast<const f16_t*>(p), 0, at.count);
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = q.get(i);
   }
@@ -157,6 +169,28 @@ __device__ __forceinline__ void drop(float* v, int col, uint32_t row, const Drop
       const float kept = v[q + i] * scale;
       v[q + i] = w[i] > last ? kept : 0.f;
     }
+  }
+}
+
+// drop() for a piece that starts anywhere: the words of the blocks it touches, moved into place.
+template <int V>
+__device__ __forceinline__ void drop_unaligned(float* v, int col, uint32_t row, const DropKey& key, uint32_t last,
+                                               float scale) {
+#pragma clang fp contract(off)
+  uint32_t w[V + 4];
+#pragma unroll
+  for (int q = 0; q < V + 4; q += 4) {
+    uint32_t b[4];
+    philox7((uint32_t)(col + q) >> 2, row, key, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[q + i] = b[i];
+  }
+  const int by = col & 3;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t word = by == 0 ? w[i] : by == 1 ? w[i + 1] : by == 2 ? w[i + 2] : w[i + 3];
+    const float kept = v[i] * scale;
+    v[i] = word > last ? kept : 0.f;
   }
 }
 

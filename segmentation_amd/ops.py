@@ -866,6 +866,7 @@ def bn_act_backward(x, dy, y, mean, var, eps, weight, want_dres):
 # ----------------------------------------------------------------------------- layer norm, dropout
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # M3D_TYPE_*
 LAYER_NORM_MAX_CHANNELS = 16384
+_MAX_ROW_STRIDE = 1 << 20   # elements; what the norms' kernels address (rows further apart are copied)
 
 
 def _scratch(nbytes: int, device) -> torch.Tensor:
@@ -876,45 +877,58 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
     return _workspace(nbytes, device)
 
 
-def _rows(t, name):
+def _here(*ts):
+    """_need_cuda for calls of a few microseconds: the check alone, and the slow path only for its message."""
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.get_device() != torch._C._cuda_getDevice()):
+            _need_cuda(*ts)
+
+
+def _addr(t):
+    """Device address as ctypes takes it for a pointer argument (a plain int; None = NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, c):
     """t [..., c] as rows for the row-wise kernels: (tensor, row stride).  Rows may lie apart (a slice of concatenated
     channels); any other layout is copied."""
-    if t.dtype not in TYPES:
-        raise TypeError(f"{name}: {t.dtype} is not supported (float32, bfloat16 or float16)")
-    c = t.shape[-1] if t.dim() else 1
-    if t.dim() == 2 and t.stride(1) == 1 and (t.stride(0) >= c or t.shape[0] == 1):
-        return t, max(t.stride(0), c)
+    if t.is_contiguous():
+        return t, c
+    if t.dim() == 2 and t.stride(1) == 1 and c <= t.stride(0) <= _MAX_ROW_STRIDE:
+        return t, t.stride(0)
     return t.contiguous(), c
 
 
 def _same_shape(name, t, shape, dtype):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
 
 
 def _norm_args(what, x, weight, bias, eps=0.0):
-    """Checks shared by the layer norms; returns (rows, channels, weight, bias, code of their type)."""
+    """Checks shared by the layer norms; returns (rows, channels, weight, bias, type of the parameters)."""
     if x.dtype not in TYPES:
         raise TypeError(f"{what}: {x.dtype} is not supported (float32, bfloat16 or float16)")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_CHANNELS:
+    c = x.shape[-1] if x.dim() else 0
+    if not 1 <= c <= LAYER_NORM_MAX_CHANNELS:
         raise ValueError(f"{what}: needs [..., c] with 1 <= c <= {LAYER_NORM_MAX_CHANNELS}, got {tuple(x.shape)}")
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
-    c = x.shape[-1]
     wdtype = None
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (c,):
+        if p.dim() != 1 or p.shape[0] != c:
             raise ValueError(f"{what}: {name} has shape {tuple(p.shape)}, expected ({c},)")
         if p.dtype not in (x.dtype, torch.float32) or (wdtype is not None and p.dtype != wdtype):
             raise TypeError(f"{what}: weight and bias are both {x.dtype} or both float32, got {name} in {p.dtype}")
         wdtype = p.dtype
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    return x.numel() // c, c, weight, bias, TYPES[wdtype or torch.float32]
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    return x.numel() // c, c, weight, bias, wdtype or torch.float32
 
 
 def _drop_args(what, p, seed, offset, state):
@@ -931,52 +945,56 @@ def _drop_args(what, p, seed, offset, state):
     return float(p), int(seed), int(offset), state
 
 
+def _like(x, dtype=None):
+    """Contiguous uninitialised tensor of x's shape."""
+    if dtype is None or dtype == x.dtype:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last axis of x [..., c] (m3d_layer_norm_fwd): returns (y, mean, rstd), y of x's shape and
     type, mean and rstd [rows] f32 for layer_norm_backward.  Float32, bfloat16 or float16; weight and bias of x's type
     or float32; rows may be strided."""
     lib = _lib.load()
     n, c, weight, bias, wtype = _norm_args("layer_norm_fwd", x, weight, bias, eps)
-    _need_cuda(x, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty((n,), dtype=torch.float32, device=x.device)
-    rstd = torch.empty((n,), dtype=torch.float32, device=x.device)
-    x, ldx = _rows(x, "x")
-    rc = lib.m3d_layer_norm_fwd(_ptr(x), ldx, TYPES[x.dtype], n, c, _ptr(weight), _ptr(bias), wtype, float(eps), _ptr(y),
-                                _ptr(mean), _ptr(rstd), _stream())
-    _lib.check(rc, "m3d_layer_norm_fwd")
+    _here(x, weight, bias)
+    y = _like(x)
+    mean, rstd = x.new_empty((2, n), dtype=torch.float32).unbind(0)
+    x, ldx = _rows(x, c)
+    rc = lib.m3d_layer_norm_fwd(x.data_ptr(), ldx, TYPES[x.dtype], n, c, _addr(weight), _addr(bias), TYPES[wtype], eps,
+                                y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _raw_stream())
+    if rc:
+        _lib.check(rc, "m3d_layer_norm_fwd")
     return y, mean, rstd
 
 
 def _stats(what, mean, rstd, n):
     for name, t in (("mean", mean), ("rstd", rstd)):
-        _same_shape(f"{what}: {name}", t, (n,), torch.float32)
+        if t.dim() != 1 or t.shape[0] != n or t.dtype != torch.float32:
+            _same_shape(f"{what}: {name}", t, (n,), torch.float32)
     return mean.contiguous(), rstd.contiguous()
-
-
-def _column_outputs(weight, wdtype, c, device, want_dweight, want_dbias):
-    dtype = wdtype if weight is None else weight.dtype
-    return (torch.empty((c,), dtype=dtype, device=device) if want_dweight else None,
-            torch.empty((c,), dtype=dtype, device=device) if want_dbias else None, TYPES[dtype])
 
 
 def layer_norm_backward(x, dy, mean, rstd, weight=None, want_dweight=True, want_dbias=True):
     """Backward of layer_norm_fwd (m3d_layer_norm_backward): returns (dx, dweight or None, dbias or None); dweight and
     dbias have the weight's type (float32 without a weight) and are summed in a fixed order."""
     lib = _lib.load()
-    n, c, weight, _, _ = _norm_args("layer_norm_backward", x, weight, None)
+    n, c, weight, _, wtype = _norm_args("layer_norm_backward", x, weight, None)
     _same_shape("layer_norm_backward: dy", dy, x.shape, x.dtype)
     mean, rstd = _stats("layer_norm_backward", mean, rstd, n)
-    _need_cuda(x, dy, mean, rstd, weight)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight, dbias, wtype = _column_outputs(weight, torch.float32, c, x.device, want_dweight, want_dbias)
+    _here(x, dy, mean, rstd, weight)
+    dx = _like(x)
+    dweight = mean.new_empty((c,), dtype=wtype) if want_dweight else None
+    dbias = mean.new_empty((c,), dtype=wtype) if want_dbias else None
     ws = _scratch(lib.m3d_layer_norm_workspace_bytes(n, c, TYPES[x.dtype]), x.device)
-    x, ldx = _rows(x, "x")
-    dy, lddy = _rows(dy, "dy")
-    rc = lib.m3d_layer_norm_backward(_ptr(x), ldx, _ptr(dy), lddy, TYPES[x.dtype], n, c, _ptr(mean), _ptr(rstd),
-                                     _ptr(weight), wtype, _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws), ws.numel(),
-                                     _stream())
-    _lib.check(rc, "m3d_layer_norm_backward")
+    x, ldx = _rows(x, c)
+    dy, lddy = _rows(dy, c)
+    rc = lib.m3d_layer_norm_backward(x.data_ptr(), ldx, dy.data_ptr(), lddy, TYPES[x.dtype], n, c, mean.data_ptr(),
+                                     rstd.data_ptr(), _addr(weight), TYPES[wtype], dx.data_ptr(), _addr(dweight),
+                                     _addr(dbias), ws.data_ptr(), ws.numel(), _raw_stream())
+    if rc:
+        _lib.check(rc, "m3d_layer_norm_backward")
     return dx, dweight, dbias
 
 
@@ -988,15 +1006,16 @@ def dropout(x, p, seed=0, offset=0, state=None):
     if x.dtype not in TYPES:
         raise TypeError(f"dropout: {x.dtype} is not supported (float32, bfloat16 or float16)")
     p, seed, offset, state = _drop_args("dropout", p, seed, offset, state)
-    _need_cuda(x, state)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _here(x, state)
+    y = _like(x)
     if x.numel() == 0:
         return y
     c = x.shape[-1] if x.dim() else 1
-    n = x.numel() // c
-    x, ldx = _rows(x, "x")
-    rc = lib.m3d_dropout(_ptr(x), ldx, TYPES[x.dtype], n, c, p, seed, offset, _ptr(state), _ptr(y), _stream())
-    _lib.check(rc, "m3d_dropout")
+    x, ldx = _rows(x, c)
+    rc = lib.m3d_dropout(x.data_ptr(), ldx, TYPES[x.dtype], x.numel() // c, c, p, seed, offset, _addr(state), y.data_ptr(),
+                         _raw_stream())
+    if rc:
+        _lib.check(rc, "m3d_dropout")
     return y
 
 
@@ -1011,12 +1030,12 @@ def dropout_next(state, step=1):
     """One call's own (seed, offset): a copy of the state, whose offset then moves on by `step` (m3d_dropout_next, one
     launch).  Both live on the device, so a captured graph draws new masks on every replay."""
     lib = _lib.load()
-    _, _, _, state = _drop_args("dropout_next", 0.0, 0, 0, state)
     if state is None:
         raise TypeError("dropout_next needs a generator state (dropout_state)")
-    _need_cuda(state)
+    _drop_args("dropout_next", 0.0, 0, 0, state)
+    _here(state)
     used = torch.empty_like(state)
-    rc = lib.m3d_dropout_next(_ptr(state), int(step), _ptr(used), _stream())
+    rc = lib.m3d_dropout_next(state.data_ptr(), int(step), used.data_ptr(), _raw_stream())
     _lib.check(rc, "m3d_dropout_next")
     return used
 
@@ -1033,25 +1052,26 @@ def dropout_add_layer_norm_fwd(x, residual, weight=None, bias=None, eps=1e-5, p=
         raise TypeError(f"{what}: the residual is {x.dtype} or float32, got {residual.dtype}")
     _same_shape(f"{what}: residual", residual, x.shape, residual.dtype)
     p, seed, offset, state = _drop_args(what, p, seed, offset, state)
-    _need_cuda(x, residual, weight, bias, state)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if want_h else None
-    mean = torch.empty((n,), dtype=torch.float32, device=x.device)
-    rstd = torch.empty((n,), dtype=torch.float32, device=x.device)
-    x, ldx = _rows(x, "x")
-    residual, ldr = _rows(residual, "residual")
-    rc = lib.m3d_dropout_add_layer_norm_fwd(_ptr(x), ldx, TYPES[x.dtype], _ptr(residual), ldr, TYPES[residual.dtype], n, c,
-                                            _ptr(weight), _ptr(bias), wtype, float(eps), p, seed, offset, _ptr(state),
-                                            _ptr(h), _ptr(y), _ptr(mean), _ptr(rstd), _stream())
-    _lib.check(rc, "m3d_dropout_add_layer_norm_fwd")
+    _here(x, residual, weight, bias, state)
+    y = _like(x)
+    h = _like(residual) if want_h else None
+    mean, rstd = x.new_empty((2, n), dtype=torch.float32).unbind(0)
+    x, ldx = _rows(x, c)
+    residual, ldr = _rows(residual, c)
+    rc = lib.m3d_dropout_add_layer_norm_fwd(x.data_ptr(), ldx, TYPES[x.dtype], residual.data_ptr(), ldr,
+                                            TYPES[residual.dtype], n, c, _addr(weight), _addr(bias), TYPES[wtype], eps, p,
+                                            seed, offset, _addr(state), _addr(h), y.data_ptr(), mean.data_ptr(),
+                                            rstd.data_ptr(), _raw_stream())
+    if rc:
+        _lib.check(rc, "m3d_dropout_add_layer_norm_fwd")
     return y, h, mean, rstd
 
 
 def dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight=None, p=0.0, seed=0, offset=0, state=None,
                                     want_dx=True, want_dresidual=True, want_dweight=True, want_dbias=True):
-    """Backward of dropout_add_layer_norm_fwd (m3d_dropout_add_layer_norm_backward): dy the gradient of y (x's
-    type), dh that of h or None; p, seed, offset and state as in the forward call.  Returns (dx, dresidual, dweight, dbias), None for what is
-    not wanted.  Without dropout dx and dresidual of one type are one tensor."""
+    """Backward of dropout_add_layer_norm_fwd (m3d_dropout_add_layer_norm_backward): dy the gradient of y (x's type), dh
+    that of h or None; p, seed, offset and state as in the forward call.  Returns (dx, dresidual, dweight, dbias), None
+    for what is not wanted.  Without dropout dx and dresidual of one type are one tensor."""
     lib = _lib.load()
     what = "dropout_add_layer_norm_backward"
     x_dtype = dy.dtype
@@ -1060,28 +1080,27 @@ def dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight=None, p=0.0, s
     _same_shape(f"{what}: dy", dy, h.shape, x_dtype)
     if dh is not None:
         _same_shape(f"{what}: dh", dh, h.shape, h.dtype)
-    n, c, weight, _, _ = _norm_args(what, dy, weight, None)
+    n, c, weight, _, wtype = _norm_args(what, dy, weight, None)
     mean, rstd = _stats(what, mean, rstd, n)
     p, seed, offset, state = _drop_args(what, p, seed, offset, state)
-    _need_cuda(h, dy, dh, mean, rstd, weight, state)
-    dev = h.device
-    one = p == 0.0 and h.dtype == x_dtype
-    dres = torch.empty(h.shape, dtype=h.dtype, device=dev) if want_dresidual or (one and want_dx) else None
-    dx = None if one or not want_dx else torch.empty(h.shape, dtype=x_dtype, device=dev)
-    dweight, dbias, wtype = _column_outputs(weight, torch.float32, c, dev, want_dweight, want_dbias)
-    if dx is None and dres is None and not (want_dweight or want_dbias):
+    _here(h, dy, dh, mean, rstd, weight, state)
+    if not (want_dx or want_dresidual or want_dweight or want_dbias):
         return None, None, None, None
-    if dx is None and dres is None:
-        dres = torch.empty(h.shape, dtype=h.dtype, device=dev)
-    ws = _scratch(lib.m3d_layer_norm_workspace_bytes(n, c, TYPES[x_dtype]), dev)
-    h, ldh = _rows(h, "h")
-    dy, lddy = _rows(dy, "dy")
-    dh, lddh = (None, 0) if dh is None else _rows(dh, "dh")
-    rc = lib.m3d_dropout_add_layer_norm_backward(_ptr(h), ldh, TYPES[h.dtype], _ptr(dy), lddy, TYPES[x_dtype], _ptr(dh),
-                                                 lddh, n, c, _ptr(mean), _ptr(rstd), _ptr(weight), wtype, p, seed, offset,
-                                                 _ptr(state), _ptr(dx), _ptr(dres), _ptr(dweight), _ptr(dbias), _ptr(ws),
-                                                 ws.numel(), _stream())
-    _lib.check(rc, "m3d_dropout_add_layer_norm_backward")
+    one = p == 0.0 and h.dtype == x_dtype
+    dx = _like(h, x_dtype) if want_dx and not one else None
+    dres = _like(h) if want_dresidual or dx is None else None
+    dweight = mean.new_empty((c,), dtype=wtype) if want_dweight else None
+    dbias = mean.new_empty((c,), dtype=wtype) if want_dbias else None
+    ws = _scratch(lib.m3d_layer_norm_workspace_bytes(n, c, TYPES[x_dtype]), h.device)
+    h, ldh = _rows(h, c)
+    dy, lddy = _rows(dy, c)
+    dh, lddh = (None, 0) if dh is None else _rows(dh, c)
+    rc = lib.m3d_dropout_add_layer_norm_backward(h.data_ptr(), ldh, TYPES[h.dtype], dy.data_ptr(), lddy, TYPES[x_dtype],
+                                                 _addr(dh), lddh, n, c, mean.data_ptr(), rstd.data_ptr(), _addr(weight),
+                                                 TYPES[wtype], p, seed, offset, _addr(state), _addr(dx), _addr(dres),
+                                                 _addr(dweight), _addr(dbias), ws.data_ptr(), ws.numel(), _raw_stream())
+    if rc:
+        _lib.check(rc, "m3d_dropout_add_layer_norm_backward")
     if one and want_dx:
         dx = dres
     return dx, dres if want_dresidual else None, dweight, dbias
