@@ -5,22 +5,22 @@
 namespace m3d {
 
 constexpr int kDropThreads = 256;
-constexpr int kDropPieces = 4;  // pieces (16 bytes) per thread
 
-// A workgroup owns kDropThreads * kDropPieces consecutive pieces of the logical [n][c] tensor; a piece is (row, piece of
+// A workgroup owns kDropThreads * U consecutive pieces (16 bytes) of the logical [n][c] tensor; a piece is (row, piece of
 // the row), the division by the pieces of a row is a multiplication (magic, shift: exact below 2^31 pieces).
-template <typename T>
+// Bound by HBM: the generator's 7 rounds are 14 widening products for 4 values, which the memory time covers.
+template <typename T, int U>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restrict__ x, int64_t ldx, int c, int64_t row0,
                                                                uint32_t total, uint32_t per_row, uint32_t magic,
                                                                int shift, DropArgs d, T* __restrict__ y) {
   constexpr int V = kPiece<T>;
   const DropKey key = drop_key(d);
-  const uint32_t base = blockIdx.x * (kDropThreads * kDropPieces) + threadIdx.x;
-  Piece<T, V> in[kDropPieces];
-  uint32_t row[kDropPieces];
-  int col[kDropPieces];
+  const uint32_t base = blockIdx.x * (kDropThreads * U) + threadIdx.x;
+  Piece<T, V> in[U];
+  uint32_t row[U];
+  int col[U];
 #pragma unroll
-  for (int u = 0; u < kDropPieces; ++u) {
+  for (int u = 0; u < U; ++u) {
     const uint32_t t = base + u * kDropThreads;
     row[u] = (__umulhi(magic, t) + t) >> shift;
     col[u] = (int)(t - row[u] * per_row) * V;
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
     else in[u].load_some(p, 0, left);
   }
 #pragma unroll
-  for (int u = 0; u < kDropPieces; ++u) {
+  for (int u = 0; u < U; ++u) {
     const uint32_t t = base + u * kDropThreads;
     float v[V];
 #pragma unroll
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
   }
 }
 
-template <typename T>
+template <typename T, int U>
 static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropArgs& d, T* y, hipStream_t stream) {
   constexpr int V = kPiece<T>;
   const uint32_t per_row = (uint32_t)cdiv(c, V);
@@ -57,11 +57,22 @@ static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropA
   for (int64_t r0 = 0; r0 < n; r0 += rows_max) {
     const int64_t rows = n - r0 < rows_max ? n - r0 : rows_max;
     const uint32_t total = (uint32_t)(rows * per_row);
-    hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)cdiv(total, kDropThreads * kDropPieces)), dim3(kDropThreads), 0,
+    hipLaunchKernelGGL((dropout_kernel<T, U>), dim3((unsigned)cdiv(total, kDropThreads * U)), dim3(kDropThreads), 0,
                        stream, x, ldx, c, r0, total, per_row, magic, shift, d, y);
     M3D_LAUNCH_CHECK();
   }
   return M3D_OK;
+}
+
+// Pieces a thread: two of whole 16-bit pieces (16384 x 4096 bf16: 47.5 us, with one 52.0, with four 47.2), one otherwise
+// (273080 x 96 f32: 35.2 us, with two 36.2, with four 39.9; 75401 x 333 f16, whose rows end inside a piece: 22.6, with
+// two 25.2).
+template <typename T>
+static int dropout_typed(const void* x, int64_t ldx, int64_t n, int c, const DropArgs& d, void* y, hipStream_t stream) {
+  const T* from = static_cast<const T*>(x);
+  if constexpr (sizeof(T) == 2)
+    if (c % kPiece<T> == 0) return dropout_launch<T, 2>(from, ldx, n, c, d, static_cast<T*>(y), stream);
+  return dropout_launch<T, 1>(from, ldx, n, c, d, static_cast<T*>(y), stream);
 }
 
 // One thread: hands a call its (seed, offset) and moves the state on.
@@ -88,11 +99,9 @@ extern "C" int m3d_dropout(const void* d_x, int64_t ldx, int type, int64_t n, in
   M3D_CHECK_ARG(ldx >= c || n == 1, "%s: row stride %lld is smaller than the %d channels", who, (long long)ldx, c);
   M3D_CHECK_ARG((((uintptr_t)d_x | (uintptr_t)d_y) & (type_bytes(type) - 1)) == 0, "%s: misaligned pointer", who);
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  if (type == M3D_TYPE_F32)
-    return dropout_launch(static_cast<const float*>(d_x), ldx, n, c, d, static_cast<float*>(d_y), stream);
-  if (type == M3D_TYPE_BF16)
-    return dropout_launch(static_cast<const bf16_t*>(d_x), ldx, n, c, d, static_cast<bf16_t*>(d_y), stream);
-  return dropout_launch(static_cast<const f16_t*>(d_x), ldx, n, c, d, static_cast<f16_t*>(d_y), stream);
+  if (type == M3D_TYPE_F32) return dropout_typed<float>(d_x, ldx, n, c, d, d_y, stream);
+  if (type == M3D_TYPE_BF16) return dropout_typed<bf16_t>(d_x, ldx, n, c, d, d_y, stream);
+  return dropout_typed<f16_t>(d_x, ldx, n, c, d, d_y, stream);
 }
 
 extern "C" int m3d_dropout_next(int64_t* d_state, int64_t step, int64_t* d_used, void* stream) {
