@@ -189,6 +189,20 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(LnArgs a) {
   }
 }
 
+// Hides from the compiler that the piece still holds what it held, so that nothing formed from it is kept in registers.
+template <typename T, int V>
+__device__ __forceinline__ void keep_packed(Piece<T, V>& q) {
+  typedef unsigned words __attribute__((ext_vector_type(V * sizeof(T) / 4)));
+  words w = __builtin_bit_cast(words, q.v);
+#pragma unroll
+  for (int i = 0; i < (int)(V * sizeof(T) / 4); ++i) {
+    unsigned one = w[i];
+    asm volatile("" : "+v"(one));
+    w[i] = one;
+  }
+  q.v = __builtin_bit_cast(typename Piece<T, V>::vec, w);
+}
+
 template <typename TX, typename TR, int K, bool ADD, bool RAGGED, int THREADS>
 __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(LnArgs a) {
   constexpr int V = kPiece<TX>;
@@ -228,11 +242,16 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(LnArgs a) {
       at.load(dy[k], k, static_cast<const TX*>(a.dy) + first * a.ld_dy, a.ld_dy, row);
     }
   };
+  // A workgroup of 1024 has 128 registers a lane: there the pieces stay packed and what the second pass needs is formed
+  // again from them, with no tile in flight (4096 x 16384 bf16 with the add: 3.3 TB/s; kept as floats and a tile ahead the
+  // spilled registers leave 2.4).
+  constexpr bool kPacked = THREADS == 1024;
   int64_t tile = blockIdx.x;
-  if (tile < a.tiles) fetch(tile);
+  if (!kPacked && tile < a.tiles) fetch(tile);
   for (; tile < a.tiles; tile += gridDim.x) {
     const int64_t first = tile * rows;
     const bool live = at.slot < a.n - first;
+    if constexpr (kPacked) fetch(tile);
     if constexpr (ADD)
       if (a.dh) {
         const int row = live ? at.slot : (int)(a.n - first) - 1;
@@ -241,28 +260,43 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_kernel(LnArgs a) {
       }
     float hat[K][V], gw[K][V], s[2] = {0.f, 0.f};
     const float scale = rstd;
+    // position i of piece k: its normalised input and the gradient behind the weight.  Neither a row behind the last one
+    // nor another lane's channel adds to a sum.
+    auto form = [&](int k, int i, float& h, float& d) {
+      h = (x[k].get(i) - mean) * rstd;
+      d = live && at.own(k, i) ? dy[k].get(i) : 0.f;
+      return d * lds[((i >> 2) * pieces + at.lane + k * at.g) * 4 + (i & 3)];
+    };
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float w = lds[((i >> 2) * pieces + at.lane + k * at.g) * 4 + (i & 3)];
-        hat[k][i] = (x[k].get(i) - mean) * rstd;
-        // neither a row behind the last one nor another lane's channel adds to a sum
-        const float d = live && at.own(k, i) ? dy[k].get(i) : 0.f;
-        gw[k][i] = d * w;
+        float d;
+        gw[k][i] = form(k, i, hat[k][i], d);
         dw[k][i] += d * hat[k][i];
         db[k][i] += d;
         s[0] += gw[k][i];
         s[1] += gw[k][i] * hat[k][i];
       }
-    if (tile + gridDim.x < a.tiles) fetch(tile + gridDim.x);
+    if (!kPacked && tile + gridDim.x < a.tiles) fetch(tile + gridDim.x);
     row_sum(s, a.lg);
     const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
+    if constexpr (kPacked) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        keep_packed(x[k]);
+        keep_packed(dy[k]);
+      }
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
+        if constexpr (kPacked) {
+          float d;
+          gw[k][i] = form(k, i, hat[k][i], d);
+        }
         v[i] = (gw[k][i] - m0 - hat[k][i] * m1) * scale;
         if constexpr (ADD)
           if (a.dh) v[i] += dh[k].get(i);
