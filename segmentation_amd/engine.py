@@ -31,7 +31,7 @@ def _fold_norm(sd: Dict[str, torch.Tensor], prefix: str, cond_idx: int, context:
                eps: float = 1e-3):
     """(scale, shift) such that PDBatchNorm_eval(x) == scale * x + shift, folded in float64."""
     key = f"{prefix}.bns.{cond_idx}" if f"{prefix}.bns.{cond_idx}.running_mean" in sd else f"{prefix}.bn"
-    if f"{key}.running_mean" not in sd and f"{prefix}.bns.{cond_idx}.weight" in sd:
+    if f"{key}.running_mean" not in sd and (f"{key}.weight" in sd or f"{prefix}.bns.{cond_idx}.weight" in sd):
         raise ValueError(f"{prefix}: the engine folds batch-norm statistics into the convolutions; a network with layer "
                          "norms (SpUNet(norm=\"layer\")) runs through spunet.SpUNet itself")
     mean = sd[f"{key}.running_mean"].double()

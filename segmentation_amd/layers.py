@@ -30,21 +30,22 @@ class _LayerNormFn(torch.autograd.Function):
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, offset, state):
-        ctx.drop = (p, seed, offset, state)
-        return ops.dropout(x, *ctx.drop)
+        ctx.drop = (p, seed, offset)
+        ctx.save_for_backward(state)
+        return ops.dropout(x, p, seed, offset, state)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return ops.dropout(dy, *ctx.drop), None, None, None, None
+        return ops.dropout(dy, *ctx.drop, *ctx.saved_tensors), None, None, None, None
 
 
 class _DropoutAddLayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, p, seed, offset, state):
         y, h, mean, rstd = ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state)
-        ctx.save_for_backward(h, weight, mean, rstd)
-        ctx.drop = dict(p=p, seed=seed, offset=offset, state=state)
+        ctx.save_for_backward(h, weight, mean, rstd, state)
+        ctx.drop = (p, seed, offset)
         ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
         return y, h
@@ -52,14 +53,13 @@ class _DropoutAddLayerNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh):
-        h, weight, mean, rstd = ctx.saved_tensors
+        h, weight, mean, rstd, state = ctx.saved_tensors
         want = ctx.needs_input_grad
         if dy is None:   # only h was used
             if dh is None:
                 return (None,) * 9
             dy = torch.zeros(h.shape, dtype=ctx.x_dtype, device=h.device)
-        grads = ops.dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight, **ctx.drop, want_dx=want[0],
-                                                    want_dresidual=want[1], want_dweight=want[2], want_dbias=want[3])
+        grads = ops.dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight, *ctx.drop, state, *want[:4])
         return (*grads, None, None, None, None, None)
 
 
@@ -121,7 +121,9 @@ class LayerNorm(nn.Module):
 class Dropout(nn.Module):
     """Dropout whose generator state is a buffer `rng` (seed, offset) on the module's device: it is saved with the
     model, and a captured graph draws a new mask on every replay.  Without a seed one is drawn from torch's generator;
-    ranks that shall draw different masks are given different seeds."""
+    ranks that shall draw different masks are given different seeds.  Every call in training moves the state on; a
+    forward that is computed twice for one backward pass (activation checkpointing) takes a `state` that the caller
+    drew once (`draw`)."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()
@@ -136,21 +138,21 @@ class Dropout(nn.Module):
         """The (seed, offset) of one call, or None where nothing is dropped."""
         return ops.dropout_next(self.rng) if self.training and self.p > 0.0 else None
 
-    def forward(self, x):
-        return dropout(x, self.p, self.training, state=self.draw())
+    def forward(self, x, state=None):
+        return dropout(x, self.p, self.training, state=self.draw() if state is None else state)
 
     def extra_repr(self):
         return f"p={self.p}"
 
 
 class DropoutAddLayerNorm(nn.Module):
-    """(x, residual) -> (y, h): h = residual + dropout(x), y = layer norm of h."""
+    """(x, residual) -> (y, h): h = residual + dropout(x), y = layer norm of h.  `state`: as in Dropout."""
 
     def __init__(self, num_features, p=0.0, eps=1e-5, affine=True, seed=None):
         super().__init__()
         self.norm = LayerNorm(num_features, eps, affine)
         self.drop = Dropout(p, seed)
 
-    def forward(self, x, residual):
+    def forward(self, x, residual, state=None):
         return dropout_add_layer_norm(x, residual, self.norm.weight, self.norm.bias, self.norm.eps, self.drop.p,
-                                      self.training, state=self.drop.draw())
+                                      self.training, state=self.drop.draw() if state is None else state)

@@ -916,19 +916,23 @@ def _norm_args(what, x, weight, bias, eps=0.0):
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
     wdtype = None
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.dim() != 1 or p.shape[0] != c:
-            raise ValueError(f"{what}: {name} has shape {tuple(p.shape)}, expected ({c},)")
-        if p.dtype not in (x.dtype, torch.float32) or (wdtype is not None and p.dtype != wdtype):
-            raise TypeError(f"{what}: weight and bias are both {x.dtype} or both float32, got {name} in {p.dtype}")
-        wdtype = p.dtype
     if weight is not None:
+        wdtype = _param_type(what, "weight", weight, c, x.dtype)
         weight = weight.contiguous()
     if bias is not None:
-        bias = bias.contiguous()
+        bdtype = _param_type(what, "bias", bias, c, x.dtype)
+        if wdtype is not None and bdtype != wdtype:
+            raise TypeError(f"{what}: weight and bias are both {x.dtype} or both float32, got bias in {bdtype}")
+        wdtype, bias = bdtype, bias.contiguous()
     return x.numel() // c, c, weight, bias, wdtype or torch.float32
+
+
+def _param_type(what, name, p, c, dtype):
+    if p.dim() != 1 or p.shape[0] != c:
+        raise ValueError(f"{what}: {name} has shape {tuple(p.shape)}, expected ({c},)")
+    if p.dtype != dtype and p.dtype != torch.float32:
+        raise TypeError(f"{what}: weight and bias are both {dtype} or both float32, got {name} in {p.dtype}")
+    return p.dtype
 
 
 def _drop_args(what, p, seed, offset, state):
@@ -943,6 +947,11 @@ def _drop_args(what, p, seed, offset, state):
         if state.dtype != torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
             raise TypeError(f"{what}: a generator state is a contiguous int64 tensor (seed, offset)")
     return float(p), int(seed), int(offset), state
+
+
+def _column(weight, like, c, dtype):
+    """Uninitialised [c] gradient of a weight or bias."""
+    return torch.empty_like(weight) if weight is not None else like.new_empty((c,), dtype=dtype)
 
 
 def _like(x, dtype=None):
@@ -985,8 +994,8 @@ def layer_norm_backward(x, dy, mean, rstd, weight=None, want_dweight=True, want_
     mean, rstd = _stats("layer_norm_backward", mean, rstd, n)
     _here(x, dy, mean, rstd, weight)
     dx = _like(x)
-    dweight = mean.new_empty((c,), dtype=wtype) if want_dweight else None
-    dbias = mean.new_empty((c,), dtype=wtype) if want_dbias else None
+    dweight = _column(weight, mean, c, wtype) if want_dweight else None
+    dbias = _column(weight, mean, c, wtype) if want_dbias else None
     ws = _scratch(lib.m3d_layer_norm_workspace_bytes(n, c, TYPES[x.dtype]), x.device)
     x, ldx = _rows(x, c)
     dy, lddy = _rows(dy, c)
@@ -1001,7 +1010,8 @@ def layer_norm_backward(x, dy, mean, rstd, weight=None, want_dweight=True, want_
 def dropout(x, p, seed=0, offset=0, state=None):
     """y = kept ? x / (1 - p) : 0 (m3d_dropout) with a mask that is a function of (seed, offset, row, channel of the last
     axis) and is never stored: the backward pass is the same call on the gradient.  state: device tensor (seed, offset)
-    int64 as dropout_next returns it, instead of `seed`; `offset` is added to the state's."""
+    int64 as dropout_next returns it, instead of `seed`; `offset` is added to the state's.  Fewer than 2^32 rows and 2^30
+    channels."""
     lib = _lib.load()
     if x.dtype not in TYPES:
         raise TypeError(f"dropout: {x.dtype} is not supported (float32, bfloat16 or float16)")
@@ -1037,6 +1047,7 @@ def dropout_next(state, step=1):
     used = torch.empty_like(state)
     rc = lib.m3d_dropout_next(state.data_ptr(), int(step), used.data_ptr(), _raw_stream())
     _lib.check(rc, "m3d_dropout_next")
+    torch.autograd.graph.increment_version(state)   # a backward pass that saved the state itself must not go on
     return used
 
 
@@ -1089,8 +1100,8 @@ def dropout_add_layer_norm_backward(h, dy, dh, mean, rstd, weight=None, p=0.0, s
     one = p == 0.0 and h.dtype == x_dtype
     dx = _like(h, x_dtype) if want_dx and not one else None
     dres = _like(h) if want_dresidual or dx is None else None
-    dweight = mean.new_empty((c,), dtype=wtype) if want_dweight else None
-    dbias = mean.new_empty((c,), dtype=wtype) if want_dbias else None
+    dweight = _column(weight, mean, c, wtype) if want_dweight else None
+    dbias = _column(weight, mean, c, wtype) if want_dbias else None
     ws = _scratch(lib.m3d_layer_norm_workspace_bytes(n, c, TYPES[x_dtype]), h.device)
     h, ldh = _rows(h, c)
     dy, lddy = _rows(dy, c)

@@ -279,6 +279,30 @@ def test_no_rows_and_other_shapes(device):
     assert torch.equal(ops.layer_norm_fwd(turned)[0], flat[:5])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_addresses_off_the_16_byte_grid(device, dtype):
+    """Slices that start at any element, and rows so far apart that the kernels do not address them (copied)."""
+    for c in (8, 24, 40, 77):
+        wide = _randn(52, 37, c + 8, dtype=dtype).to(device)
+        for s in range(8):
+            x, r = wide[:, s:s + c], wide[:, 8 - s:8 - s + c]
+            xc, rc = x.contiguous(), r.contiguous()
+            y, h, mean, rstd = ops.dropout_add_layer_norm_fwd(x, r, p=0.25, seed=s)
+            want = ops.dropout_add_layer_norm_fwd(xc, rc, p=0.25, seed=s)
+            assert all(torch.equal(a, b) for a, b in zip((y, h, mean, rstd), want))
+            got = ops.dropout_add_layer_norm_backward(h, x, r, mean, rstd, p=0.25, seed=s)
+            assert all(torch.equal(a, b) for a, b in zip(got, ops.dropout_add_layer_norm_backward(h, xc, rc, mean, rstd,
+                                                                                                  p=0.25, seed=s)))
+            assert torch.equal(ops.layer_norm_fwd(x)[0], ops.layer_norm_fwd(xc)[0])
+            assert torch.equal(ops.dropout(x, 0.25, s), ops.dropout(xc, 0.25, s))
+            w = wide.flatten()[s:s + c]   # a weight off the grid
+            assert torch.equal(ops.layer_norm_fwd(xc, w, w)[0], ops.layer_norm_fwd(xc, w.clone(), w.clone())[0])
+    far = torch.zeros(3, (1 << 20) + 40, dtype=dtype, device=device)
+    far[:, :77] = wide[:3, :77]
+    assert torch.equal(ops.layer_norm_fwd(far[:, :77])[0], ops.layer_norm_fwd(wide[:3, :77].contiguous())[0])
+    assert torch.equal(ops.dropout(far[:, :77], 0.5, 3), ops.dropout(wide[:3, :77].contiguous(), 0.5, 3))
+
+
 def test_rows_behind_the_last_are_left_alone(device):
     """The kernels write their own rows and channels, nothing behind them."""
     import ctypes
@@ -395,6 +419,24 @@ def test_generator_state(device):
     m2.load_state_dict(m.state_dict())
     assert torch.equal(m2(x), m(x))
     assert m.eval()(x) is x
+
+
+def test_a_state_that_moved_on_is_refused(device):
+    """A backward pass whose mask can no longer be formed says so; a drawn state is the caller's to keep, and serves a
+    forward that is computed twice (activation checkpointing)."""
+    from torch.utils.checkpoint import checkpoint
+    x = _randn(102, 40, 24).to(device).requires_grad_()
+    st = ops.dropout_state(5, device)
+    for y in (layers.dropout(x, 0.5, state=st), layers.dropout_add_layer_norm(x, x, p=0.5, state=st)[0]):
+        ops.dropout_next(st)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    block = layers.DropoutAddLayerNorm(24, 0.5, seed=9).to(device)
+    gy = _randn(103, 40, 24).to(device)
+    st = block.drop.draw()
+    direct = torch.autograd.grad((block(x, x, st)[0] * gy).sum(), x)[0]
+    again = torch.autograd.grad((checkpoint(lambda t: block(t, t, st)[0], x, use_reentrant=False) * gy).sum(), x)[0]
+    assert torch.equal(direct, again) and block.drop.rng.tolist() == [9, 1]
 
 
 def test_block_in_a_captured_graph(device):

@@ -105,7 +105,7 @@ def test_refusals_of_the_entry_points():
         return lib.m3d_layer_norm_fwd(x, ld, typ, n, c, w, null, wt, eps, y, one, one, null)
 
     for bad in (dict(typ=3), dict(wt=2), dict(c=0), dict(c=16385), dict(n=-1), dict(n=1 << 32), dict(x=null), dict(y=null),
-                dict(x=odd), dict(w=odd), dict(ld=7), dict(eps=-1.0), dict(eps=float("nan"))):
+                dict(x=odd), dict(w=odd), dict(ld=7), dict(ld=(1 << 20) + 1), dict(eps=-1.0), dict(eps=float("nan"))):
         assert fwd(**bad) == -1 and lib.m3d_last_error(), bad
     assert fwd(n=0) == 0
 
@@ -175,3 +175,6 @@ def test_layer_norm_backbone_is_built_and_refused_by_the_engine():
     sd = {"backbone." + k: v for k, v in net.state_dict().items()}
     with pytest.raises(ValueError, match="batch-norm statistics"):
         engine._fold_norm(sd, "backbone.conv_input.bn", 0, torch.zeros(1, 256))
+    one = spunet.SpUNet(norm="layer", norm_decouple=False, norm_adaptive=False, **kw)
+    with pytest.raises(ValueError, match="batch-norm statistics"):
+        engine._fold_norm(one.state_dict(), "conv_input.bn", 0, None)
