@@ -7,9 +7,10 @@ namespace m3d {
 constexpr int kDropThreads = 256;
 
 // A workgroup owns kDropThreads * U consecutive pieces (16 bytes) of the logical [n][c] tensor; a piece is (row, piece of
-// the row), the division by the pieces of a row is a multiplication (magic, shift: exact below 2^31 pieces).
+// the row), the division by the pieces of a row is a multiplication (magic, shift: exact below 2^31 pieces).  WHOLE: no row
+// ends inside a piece.
 // Bound by HBM: the generator's 7 rounds are 14 widening products for 4 values, which the memory time covers.
-template <typename T, int U>
+template <typename T, int U, bool WHOLE>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restrict__ x, int64_t ldx, int c, int64_t row0,
                                                                uint32_t total, uint32_t per_row, uint32_t magic,
                                                                int shift, DropArgs d, T* __restrict__ y) {
@@ -26,8 +27,13 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
     col[u] = (int)(t - row[u] * per_row) * V;
     const T* p = x + (row0 + row[u]) * ldx + col[u];
     const int left = t < total ? c - col[u] : 0;
-    if (left >= V) in[u].load(p);
-    else in[u].load_some(p, 0, left);
+    if constexpr (WHOLE) {
+      if (left > 0) in[u].load_stream(p);
+    } else if (left >= V) {
+      in[u].load(p);
+    } else {
+      in[u].load_some(p, 0, left);
+    }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -41,11 +47,11 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restri
     T* p = y + (row0 + row[u]) * c + col[u];
     const int left = t < total ? c - col[u] : 0;
     if (left >= V) in[u].store(p);
-    else in[u].store_some(p, 0, left);
+    else if constexpr (!WHOLE) in[u].store_some(p, 0, left);
   }
 }
 
-template <typename T, int U>
+template <typename T, int U, bool WHOLE>
 static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropArgs& d, T* y, hipStream_t stream) {
   constexpr int V = kPiece<T>;
   const uint32_t per_row = (uint32_t)cdiv(c, V);
@@ -57,7 +63,7 @@ static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropA
   for (int64_t r0 = 0; r0 < n; r0 += rows_max) {
     const int64_t rows = n - r0 < rows_max ? n - r0 : rows_max;
     const uint32_t total = (uint32_t)(rows * per_row);
-    hipLaunchKernelGGL((dropout_kernel<T, U>), dim3((unsigned)cdiv(total, kDropThreads * U)), dim3(kDropThreads), 0,
+    hipLaunchKernelGGL((dropout_kernel<T, U, WHOLE>), dim3((unsigned)cdiv(total, kDropThreads * U)), dim3(kDropThreads), 0,
                        stream, x, ldx, c, r0, total, per_row, magic, shift, d, y);
     M3D_LAUNCH_CHECK();
   }
@@ -70,9 +76,9 @@ static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropA
 template <typename T>
 static int dropout_typed(const void* x, int64_t ldx, int64_t n, int c, const DropArgs& d, void* y, hipStream_t stream) {
   const T* from = static_cast<const T*>(x);
-  if constexpr (sizeof(T) == 2)
-    if (c % kPiece<T> == 0) return dropout_launch<T, 2>(from, ldx, n, c, d, static_cast<T*>(y), stream);
-  return dropout_launch<T, 1>(from, ldx, n, c, d, static_cast<T*>(y), stream);
+  if (c % kPiece<T> == 0)
+    return dropout_launch<T, sizeof(T) == 2 ? 2 : 1, true>(from, ldx, n, c, d, static_cast<T*>(y), stream);
+  return dropout_launch<T, 1, false>(from, ldx, n, c, d, static_cast<T*>(y), stream);
 }
 
 // One thread: hands a call its (seed, offset) and moves the state on.

@@ -87,7 +87,8 @@ struct Lane {
   __device__ __forceinline__ void load(Piece<T, V>& q, int k, const T* base, int64_t ld, int row) const {
     const Place p = at(k);
     const uint32_t off = (uint32_t)row * (uint32_t)ld + (uint32_t)p.col;
-    if (RAGGED && p.count < V) q.load_some(base + off, 0, p.count);
+    if constexpr (!RAGGED) q.load_stream(base + off);
+    else if (p.count < V) q.load_some(base + off, 0, p.count);
     else q.load(base + off);
   }
   template <typename T>
