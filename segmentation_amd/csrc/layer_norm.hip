@@ -11,6 +11,11 @@
 // lane permutations, wider rows take a group of several waves that add through LDS.  All sums are f32.
 // The column sums of the backward pass stay in registers over all rows of a workgroup, are joined inside it, written as
 // one partial row per workgroup and added up by a second launch in a fixed order (no atomics: run-to-run identical).
+//
+// Bound by HBM: 2 values moved for each forward, 3 for each backward (4 and 5 with the add), about 20 operations a value.
+// Kernel times, with 2 x FETCH_SIZE + WRITE_SIZE within 2 % of those bytes: 273080 x 96 f32 35.7 us forward (5.9 TB/s),
+// 54.2 backward (5.8); 75401 x 768 bf16 39.9 and 59.8 (5.8); 16384 x 4096 bf16 with dropout and add 99.5 (5.4) and 124.3
+// (5.4); the join of the columns 4.8.  A copy of 1 GB runs at 5.2.
 #include "rowops.h"
 
 namespace m3d {

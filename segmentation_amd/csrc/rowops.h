@@ -127,7 +127,8 @@ __device__ __forceinline__ float group_sum(float v, int g) {
 
 // ---------------------------------------------------------------- dropout masks
 // Philox 4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with 7 rounds, the
-// fewest that pass its authors' whole test battery.  A block of four 32-bit words belongs to four consecutive channels
+// fewest that pass its authors' whole test battery (with 10, 16384 x 4096 bf16 values take 58 us instead of 48.6: the
+// products, not the memory, bound them).  A block of four 32-bit words belongs to four consecutive channels
 // of a row: counter = (channel / 4, row, offset low, offset high), key = seed.  A value is kept where its word is at
 // least p * 2^32, so the mask is a function of (seed, offset, row, channel) alone, whatever the type, stride or kernel.
 struct DropArgs {
