@@ -573,6 +573,23 @@ def test_offsets_beyond_32_bits(device):
     assert torch.equal(z[-1].cpu() != 0, last & (tail[-1].cpu() != 0))
 
 
+def test_more_rows_than_31_bits(device):
+    """2^31 + 100 rows of one channel: several launches of the dropout, 64-bit rows in the norm."""
+    n = 2 ** 31 + 100
+    x = torch.ones(n, 1, dtype=BF16, device=device)
+    y = ops.dropout(x, 0.5, 7, 8)
+    for lo in (0, 0x7fff0000 - 50, n - 100):
+        words = O.philox4x32((0, np.arange(lo, lo + 100), 8, 0), (7, 0), 7)[0]
+        keep = torch.from_numpy(words.astype(np.int64) >= 2 ** 31)
+        assert torch.equal(y[lo:lo + 100, 0].cpu() == 2, keep) and torch.equal(y[lo:lo + 100, 0].cpu() == 0, ~keep)
+    x[-1] = 5
+    b = torch.full((1,), 0.25, dtype=BF16, device=device)
+    del y
+    y, mean, rstd = ops.layer_norm_fwd(x, None, b)
+    assert mean[-2:].tolist() == [1.0, 5.0] and y[-1].item() == 0.25 and y[2 ** 30].item() == 0.25
+    del y, rstd
+
+
 def test_tensors_of_a_wrong_place_are_refused(device):
     x = torch.zeros(4, 8, device=device)
     with pytest.raises(RuntimeError, match="no CPU path"):
