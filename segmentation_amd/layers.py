@@ -87,16 +87,16 @@ def dropout(x, p=0.5, training=True, seed=0, offset=0, state=None):
 
 
 def dropout_add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, training=True, seed=0, offset=0,
-                           state=None):
+                           state=None, need_h=True):
     """(y, h) with h = residual + dropout(x) and y = layer norm of h (ops.dropout_add_layer_norm_fwd), differentiable in
     x, residual, weight and bias through both outputs; no dropout outside training.  The residual stream is of x's type or
-    float32."""
+    float32.  need_h=False: the caller goes on with y alone (post-norm blocks); h is None where no gradient needs it."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} is not in [0, 1]")
     if not training or p == 0.0:
         p, seed, offset, state = 0.0, 0, 0, None
     if not _taped(x, residual, weight, bias):
-        return ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state)[:2]
+        return ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state, need_h)[:2]
     return _DropoutAddLayerNormFn.apply(x, residual, weight, bias, eps, p, seed, offset, state)
 
 

@@ -101,7 +101,7 @@ class PDLayerNorm(PDBatchNorm):
         else:
             state = self.drop.draw() if self.drop is not None else None
             p = self.drop.p if state is not None else 0.0
-            y, _ = layers.dropout_add_layer_norm(feat, residual, weight, bias, norm.eps, p, state=state)
+            y, _ = layers.dropout_add_layer_norm(feat, residual, weight, bias, norm.eps, p, state=state, need_h=False)
         return F.relu(y) if relu else y
 
     def _modulated(self, norm, feat, scale, shift, residual, relu):

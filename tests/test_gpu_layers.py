@@ -178,6 +178,8 @@ def test_dropout_add_layer_norm(device, n, c, p, xt, rt, wt):
             tw, tb = _tol_columns(HD, DY, MEAN, RSTD)
             _close("dw", dw, DW, tw + _half(wt, DW.abs() + tw))
             _close("db", db, DB, tb + _half(wt, DB.abs() + tb))
+    with torch.inference_mode():   # (tensors made here have no version)
+        ops.dropout_next(ops.dropout_state(1, device))
     bare = ops.dropout_add_layer_norm_fwd(x.to(device), r.to(device), wg, bg, want_h=False, **kw)
     assert bare[1] is None and torch.equal(bare[0], y)
     only = ops.dropout_add_layer_norm_backward(h, dy.to(device), None, mean, rstd, wg, want_dresidual=False,
@@ -639,6 +641,45 @@ def test_backbone_with_layer_norms(device):
     d.square().mean().backward()
     used = [(k, p) for k, p in net.named_parameters() if ".bns." not in k or ".bns.0." in k]
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for _, p in used)
+
+
+@pytest.mark.parametrize("decouple,adaptive,affine", [(True, True, True), (True, True, False), (False, False, True),
+                                                      (False, True, True), (True, False, False)])
+@pytest.mark.parametrize("with_res,relu", [(False, False), (True, True)])
+def test_pd_layer_norm_matches_float64(device, decouple, adaptive, affine, with_res, relu):
+    """relu?(layer norm(residual + x) (1 + scale) + shift) with its gradients, every combination of the options.  Bars as
+    for the batch norms: relative 2-norm 1e-5 of outputs and input gradients, 1e-4 of parameters."""
+    torch.manual_seed(8)
+    m = spunet.PDLayerNorm(48, 32, decouple=decouple, adaptive=adaptive, affine=affine)
+    for p in m.parameters():
+        p.data.normal_(0.0, 0.3)
+    ref = copy.deepcopy(m).double()
+    m = m.to(device)
+    x, res, ctx, gy = _randn(151, 90, 48), _randn(152, 90, 48), _randn(153, 1, 32), _randn(154, 90, 48)
+    ins = [t.to(device).requires_grad_() for t in (x, res, ctx)]
+    y = m(ins[0], "Matterport3D", ins[2], residual=ins[1] if with_res else None, relu=relu)
+    X, R, C = (t.double().requires_grad_() for t in (x, res, ctx))
+    H = X + R if with_res else X
+    D = H - H.mean(1, keepdim=True)
+    Y = D * (D.square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    ln = ref.bns[2] if decouple else ref.bn
+    if affine:
+        Y = Y * ln.weight + ln.bias
+    if adaptive:
+        shift, scale = ref.modulation(C).chunk(2, dim=1)
+        Y = Y * (1.0 + scale) + shift
+    if relu:
+        gy = gy * (Y.detach().abs() > 1e-4).float()   # no gradient within rounding distance of the kink
+        Y = Y.clamp_min(0)
+    y.backward(gy.to(device))
+    Y.backward(gy.double())
+    rel = lambda a, b: float((a.detach().double().cpu() - b).norm() / b.norm())
+    assert rel(y, Y.detach()) < 1e-5 and rel(ins[0].grad, X.grad) < 1e-5
+    assert not with_res or rel(ins[1].grad, R.grad) < 1e-5
+    for (k, p), (_, q) in zip(m.named_parameters(), ref.named_parameters()):
+        assert (p.grad is None) == (q.grad is None), k
+        assert q.grad is None or rel(p.grad, q.grad) < 1e-4, k
+    assert not adaptive or rel(ins[2].grad, C.grad) < 1e-4
 
 
 def test_optimisation_step_with_layer_norms(device):
