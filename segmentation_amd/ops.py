@@ -877,11 +877,16 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
     return _workspace(nbytes, device)
 
 
-def _here(*ts):
+def _here(x, *ts):
     """_need_cuda for calls of a few microseconds: the check alone, and the slow path only for its message."""
+    if not x.is_cuda:
+        _need_cuda(x)
+    dev = torch._C._cuda_getDevice()
+    if x.get_device() != dev:
+        _need_cuda(x)
     for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != torch._C._cuda_getDevice()):
-            _need_cuda(*ts)
+        if t is not None and t.get_device() != dev:
+            _need_cuda(t)
 
 
 def _addr(t):
@@ -908,31 +913,30 @@ def _same_shape(name, t, shape, dtype):
 
 def _norm_args(what, x, weight, bias, eps=0.0):
     """Checks shared by the layer norms; returns (rows, channels, weight, bias, type of the parameters)."""
-    if x.dtype not in TYPES:
-        raise TypeError(f"{what}: {x.dtype} is not supported (float32, bfloat16 or float16)")
-    c = x.shape[-1] if x.dim() else 0
+    dtype = x.dtype
+    if dtype not in TYPES:
+        raise TypeError(f"{what}: {dtype} is not supported (float32, bfloat16 or float16)")
+    c = x.size(-1) if x.dim() else 0
     if not 1 <= c <= LAYER_NORM_MAX_CHANNELS:
         raise ValueError(f"{what}: needs [..., c] with 1 <= c <= {LAYER_NORM_MAX_CHANNELS}, got {tuple(x.shape)}")
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
-    wdtype = None
+    wdtype = torch.float32
     if weight is not None:
-        wdtype = _param_type(what, "weight", weight, c, x.dtype)
-        weight = weight.contiguous()
+        wdtype = weight.dtype
+        weight = _param(what, "weight", weight, c, dtype, wdtype)
     if bias is not None:
-        bdtype = _param_type(what, "bias", bias, c, x.dtype)
-        if wdtype is not None and bdtype != wdtype:
-            raise TypeError(f"{what}: weight and bias are both {x.dtype} or both float32, got bias in {bdtype}")
-        wdtype, bias = bdtype, bias.contiguous()
-    return x.numel() // c, c, weight, bias, wdtype or torch.float32
+        bias = _param(what, "bias", bias, c, dtype, wdtype if weight is not None else bias.dtype)
+        wdtype = bias.dtype
+    return x.numel() // c, c, weight, bias, wdtype
 
 
-def _param_type(what, name, p, c, dtype):
-    if p.dim() != 1 or p.shape[0] != c:
+def _param(what, name, p, c, dtype, wdtype):
+    if p.dim() != 1 or p.numel() != c:
         raise ValueError(f"{what}: {name} has shape {tuple(p.shape)}, expected ({c},)")
-    if p.dtype != dtype and p.dtype != torch.float32:
+    if p.dtype != wdtype or (wdtype != dtype and wdtype != torch.float32):
         raise TypeError(f"{what}: weight and bias are both {dtype} or both float32, got {name} in {p.dtype}")
-    return p.dtype
+    return p if p.is_contiguous() else p.contiguous()
 
 
 def _drop_args(what, p, seed, offset, state):
@@ -956,9 +960,9 @@ def _column(weight, like, c, dtype):
 
 def _like(x, dtype=None):
     """Contiguous uninitialised tensor of x's shape."""
-    if dtype is None or dtype == x.dtype:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
-    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+    if dtype is not None:
+        return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
