@@ -345,11 +345,12 @@ size_t m3d_bn_stats_static_max_bytes(void);
 int m3d_bn_stats_static(const float* d_x, int64_t n, int c, float* d_mean, float* d_var, void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * Layer norm, dropout, and the residual add that joins them, on [n, c] activations of type M3D_TYPE_F32 / _BF16 / _F16
- * (0 <= n < 2^32 rows, 1 <= c <= 16384 channels for the norms; any channel count and row stride ld* >= c in elements,
- * any address a multiple of the element size).  They are nn.LayerNorm and nn.Dropout of the reference's transformer
- * decoder on point features (mosaic3d/src/models/networks/opensegment3d).  Outputs are contiguous; weight and bias
- * (`wtype`: f32 or the activations' type) may be NULL (1 and 0).  Sums are f32, each output is rounded once.
+ * Layer norm, dropout, and the residual add that joins them, on [n, c] activations of type M3D_TYPE_F32 / _BF16 / _F16:
+ * 0 <= n < 2^32 rows; 1 <= c <= 16384 channels and row strides c <= ld* <= 2^20 (in elements) for the norms, c < 2^30 and
+ * any ldx >= c for m3d_dropout; any address that is a multiple of the element size.  They are nn.LayerNorm and nn.Dropout
+ * of the reference's transformer decoder on point features (mosaic3d/src/models/networks/opensegment3d).  Outputs are
+ * contiguous; weight and bias (`wtype`: f32 or the activations' type) may be NULL (1 and 0).  Sums are f32, each output is
+ * rounded once.
  *
  *   m3d_layer_norm_fwd:       y = (x - mean) * rstd * weight + bias;  d_mean[n], d_rstd[n] (f32) = mean and
  *                             1 / sqrt(biased variance + eps) of the row, for the backward pass
