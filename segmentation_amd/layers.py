@@ -123,7 +123,7 @@ class Dropout(nn.Module):
     model, and a captured graph draws a new mask on every replay.  Without a seed one is drawn from torch's generator;
     ranks that shall draw different masks are given different seeds.  Every call in training moves the state on; a
     forward that is computed twice for one backward pass (activation checkpointing) takes a `state` that the caller
-    drew once (`draw`)."""
+    drew once (`draw`), and a draw inside the recomputation is refused: it would be another mask."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()
@@ -136,7 +136,14 @@ class Dropout(nn.Module):
 
     def draw(self):
         """The (seed, offset) of one call, or None where nothing is dropped."""
-        return ops.dropout_next(self.rng) if self.training and self.p > 0.0 else None
+        if not (self.training and self.p > 0.0):
+            return None
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("dropout: a mask is drawn inside a backward pass, by a forward that is recomputed "
+                               "(activation checkpointing); its gradients would belong to another mask than its result.  "
+                               "Draw the state in front of the checkpointed call and hand it in (state=, or "
+                               "dropout_states= of SpUNet)")
+        return ops.dropout_next(self.rng)
 
     def forward(self, x, state=None):
         return dropout(x, self.p, self.training, state=self.draw() if state is None else state)

@@ -91,6 +91,16 @@ class PDLayerNorm(PDBatchNorm):
                          affine=affine)
         self.drop = layers.Dropout(dropout) if dropout > 0.0 else None
 
+    def forward(self, feat, condition=None, context=None, residual=None, relu=False, state=None):
+        """`state`: what `drop.draw()` returned, for a call that is computed twice (activation checkpointing); None: the
+        call draws its own."""
+        if state is not None:
+            self.__dict__["_state"] = state
+        try:
+            return super().forward(feat, condition, context, residual, relu)
+        finally:
+            self.__dict__.pop("_state", None)
+
     @staticmethod
     def _make_norm(num_features, eps, momentum, affine):
         return layers.LayerNorm(num_features, affine=affine)
@@ -99,7 +109,11 @@ class PDLayerNorm(PDBatchNorm):
         if residual is None:
             y = layers.layer_norm(feat, weight, bias, norm.eps)
         else:
-            state = self.drop.draw() if self.drop is not None else None
+            state = self.__dict__.pop("_state", None)   # set for one call by forward or SpUNet.forward
+            if self.drop is None or not self.drop.training:
+                state = None
+            elif state is None:
+                state = self.drop.draw()
             p = self.drop.p if state is not None else 0.0
             y, _ = layers.dropout_add_layer_norm(feat, residual, weight, bias, norm.eps, p, state=state, need_h=False)
         return F.relu(y) if relu else y
@@ -341,13 +355,29 @@ class SpUNet(nn.Module):
         for m, w, b in zip(norms, weight.split(sizes), bias.split(sizes)):
             m.__dict__["_affine"] = (w, b)
 
+    def _dropping_norms(self):
+        """The norms that drop: those behind the residual add of a block."""
+        return [m.bn2 for m in self.modules() if isinstance(m, BasicBlock) and getattr(m.bn2, "drop", None) is not None]
+
+    def draw_dropout(self):
+        """The generator states of one forward, one for each block: input_dict["dropout_states"] of a forward that is
+        computed twice for one backward pass (activation checkpointing), drawn in front of it."""
+        return [m.drop.draw() for m in self._dropping_norms()]
+
     def forward(self, input_dict):
         """Returns dict(sparse_conv_feat, feat [N0, out], v2p_map [N_pts]) -- the fields of the
-        reference's Point that the head reads (language_module.py:202-207)."""
+        reference's Point that the head reads (language_module.py:202-207).  input_dict["dropout_states"]: as draw_dropout
+        returned them; without it every block draws its own."""
+        states = input_dict.get("dropout_states")
+        dropping = self._dropping_norms() if states is not None else []
+        if states is not None and len(states) != len(dropping):
+            raise ValueError(f"dropout_states holds {len(states)} states, the network drops in {len(dropping)} blocks")
         x, vox = self.sparsify(input_dict)
         condition = input_dict["condition"][0]
         context = input_dict.get("context")
         try:
+            for m, state in zip(dropping, states or ()):
+                m.__dict__["_state"] = state
             self._fold_modulations(condition, context, x.features.dtype)
             return self._forward_net(x, vox, condition, context)
         finally:
@@ -355,6 +385,8 @@ class SpUNet(nn.Module):
             # behind for the next call (or for a direct call of a sub-module)
             for m in self.__dict__.get("_pd_norms") or ():
                 m.__dict__.pop("_affine", None)
+            for m in dropping:
+                m.__dict__.pop("_state", None)
 
     def _forward_net(self, x, vox, condition, context):
         x = self.conv_input([x, condition, context])

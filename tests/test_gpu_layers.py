@@ -698,3 +698,28 @@ def test_optimisation_step_with_layer_norms(device):
     moved = [k for k, p in net.named_parameters() if not torch.equal(p, before[k])]
     assert all(torch.isfinite(p).all() for p in net.parameters())
     assert any(".bns.0.weight" in k for k in moved) and any("conv2.weight" in k for k in moved)
+
+
+def test_checkpointed_backbone_with_dropout(device):
+    """The whole network under activation checkpointing: refused where its blocks draw for themselves, and with states
+    that were drawn in front of it the gradients of the plain call with those states (bar: the order of the sums of the
+    convolutions' gradients, relative 2-norm 1e-4 as for parameters above)."""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(9)
+    net = spunet.PPT(spunet.SpUNet(channels=(32, 64, 64, 32), layers=(1, 1, 1, 1), out_channels=32, norm="layer",
+                                   dropout=0.3)).to(device)
+    batch = _batch(device)
+    params = [p for k, p in net.named_parameters() if "conv2.weight" in k]
+    feat = batch.pop("feat").requires_grad_()
+    run = lambda f, **kw: net(dict(batch, feat=f, **kw))["feat"].square().mean()
+    with pytest.raises(RuntimeError, match="inside a backward pass"):
+        checkpoint(run, feat, use_reentrant=False).backward()
+    states = net.backbone.draw_dropout()
+    want = torch.autograd.grad(run(feat, dropout_states=states), params)
+    other = torch.autograd.grad(run(feat), params)   # masks of its own
+    counts = [m.drop.rng[1].item() for m in net.backbone._dropping_norms()]
+    got = torch.autograd.grad(checkpoint(lambda f: run(f, dropout_states=states), feat, use_reentrant=False), params)
+    assert counts == [m.drop.rng[1].item() for m in net.backbone._dropping_norms()]
+    rel = lambda a, b: float((a.double() - b.double()).norm() / b.double().norm())
+    assert all(rel(a, b) < 1e-4 for a, b in zip(got, want))
+    assert any(rel(a, b) > 1e-2 for a, b in zip(other, want))

@@ -178,3 +178,96 @@ def test_layer_norm_backbone_is_built_and_refused_by_the_engine():
     one = spunet.SpUNet(norm="layer", norm_decouple=False, norm_adaptive=False, **kw)
     with pytest.raises(ValueError, match="batch-norm statistics"):
         engine._fold_norm(one.state_dict(), "conv_input.bn", 0, None)
+
+
+# ---------------------------------------------------------------- modules over stand-ins of the kernels' definitions
+@pytest.fixture
+def definitions(monkeypatch):
+    """ops.* of this family on the CPU, from the float64 formulas and the generator's definition; `calls` of the dropout
+    functions: (p, seed, offset, state)."""
+    calls = []
+
+    def keep(x, p, seed, offset, state):
+        calls.append((p, seed, offset, None if state is None else state.tolist()))
+        if state is not None:
+            seed, offset = int(state[0]), offset + int(state[1])
+        n, c = x.numel() // x.shape[-1], x.shape[-1]
+        return O.dropout(torch.ones(n, c, dtype=torch.float64), p, seed, offset).reshape(x.shape)
+
+    def next_state(state, step=1):
+        used = state.clone()
+        state[1] += step
+        return used
+
+    def drop(x, p, seed=0, offset=0, state=None):
+        return (x.double() * keep(x, p, seed, offset, state)).to(x.dtype)
+
+    def norm(x, weight=None, bias=None, eps=1e-5):
+        y, mean, rstd = O.layer_norm(x.double(), weight, bias, eps)
+        return y.to(x.dtype).detach(), mean.detach(), rstd.detach()
+
+    def norm_back(x, dy, mean, rstd, weight=None, want_dweight=True, want_dbias=True):
+        dx, dw, db = O.layer_norm_backward(x.double(), dy.double(), mean, rstd, weight)
+        return dx.to(x.dtype), dw.to(x.dtype) if want_dweight else None, db.to(x.dtype) if want_dbias else None
+
+    def add(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0, state=None, want_h=True):
+        h = (residual.double() + x.double() * keep(x, p, seed, offset, state)).to(residual.dtype)
+        y, mean, rstd = norm(h, weight, bias, eps)
+        return y.to(x.dtype), h.detach() if want_h else None, mean, rstd
+
+    def add_back(h, dy, dh, mean, rstd, weight=None, p=0.0, seed=0, offset=0, state=None, want_dx=True,
+                 want_dresidual=True, want_dweight=True, want_dbias=True):
+        t, dw, db = norm_back(h, dy, mean, rstd, weight, want_dweight, want_dbias)
+        t = t if dh is None else t + dh
+        dx = (t.double() * keep(t, p, seed, offset, state)).to(dy.dtype)
+        return dx if want_dx else None, t if want_dresidual else None, dw, db
+
+    for name, fn in (("dropout", drop), ("dropout_next", next_state), ("layer_norm_fwd", norm),
+                     ("layer_norm_backward", norm_back), ("dropout_add_layer_norm_fwd", add),
+                     ("dropout_add_layer_norm_backward", add_back)):
+        monkeypatch.setattr(ops, name, fn)
+    return calls
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_forward_does_not_draw(definitions, reentrant):
+    """Under activation checkpointing a module that draws for itself is refused; a state that was drawn in front of the
+    call gives the gradients of the plain call, and the generator moves on once."""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(1)
+    x, r = torch.randn(20, 16, requires_grad=True), torch.randn(20, 16, requires_grad=True)
+    gy = torch.randn(20, 16)
+    norm = spunet.PDLayerNorm(16, 4, dropout=0.5)
+    block, drop = layers.DropoutAddLayerNorm(16, 0.5, seed=3), layers.Dropout(0.5, seed=4)
+    forms = [(norm.drop, lambda a, b, st: norm(a, "ScanNet", residual=b, relu=True, state=st)),
+             (block.drop, lambda a, b, st: block(a, b, st)[0]),
+             (drop, lambda a, b, st: drop(a, st) + b)]
+    for module, form in forms:
+        y = checkpoint(lambda a, b: form(a, b, None), x, r, use_reentrant=reentrant)
+        with pytest.raises(RuntimeError, match="inside a backward pass"):
+            (y * gy).sum().backward()
+        before = module.rng.clone()
+        st = module.draw()
+        want = torch.autograd.grad((form(x, r, st) * gy).sum(), (x, r))
+        x.grad = r.grad = None
+        (checkpoint(lambda a, b: form(a, b, st), x, r, use_reentrant=reentrant) * gy).sum().backward()
+        assert torch.equal(x.grad, want[0]) and torch.equal(r.grad, want[1]) and want[0].abs().sum() > 0
+        assert module.rng.tolist() == [before[0].item(), before[1].item() + 1]
+        x.grad = r.grad = None
+        (form(x, r, None) * gy).sum().backward()   # a plain call draws its own, in front of its backward pass
+    norm.eval()
+    assert torch.equal(norm(x, "ScanNet", residual=r, state=st), norm(x, "ScanNet", residual=r))
+    assert "_state" not in norm.__dict__
+
+
+def test_network_states_are_drawn_and_counted():
+    kw = dict(channels=(32, 64, 64, 32), layers=(1, 1, 1, 1), out_channels=32)
+    net = spunet.SpUNet(norm="layer", dropout=0.1, **kw)
+    blocks = [m for m in net.modules() if isinstance(m, spunet.BasicBlock)]
+    assert net._dropping_norms() == [b.bn2 for b in blocks] and len(blocks) == 4
+    assert net.eval().draw_dropout() == [None] * 4
+    assert spunet.SpUNet(norm="layer", **kw).draw_dropout() == [] and spunet.SpUNet(**kw).draw_dropout() == []
+    with pytest.raises(ValueError, match="drops in 4 blocks"):
+        net(dict(dropout_states=[None] * 3))
+    with pytest.raises(ValueError, match="drops in 0 blocks"):
+        spunet.SpUNet(**kw)(dict(dropout_states=[None]))
