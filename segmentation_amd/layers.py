@@ -3,9 +3,10 @@ ops.layer_norm_fwd, ops.dropout and ops.dropout_add_layer_norm_fwd: what a trans
 of around its matrix products (nn.LayerNorm and nn.Dropout in mosaic3d/src/models/networks/opensegment3d).
 
 Activations [..., c] in float32, bfloat16 or float16, weight and bias in the same type or float32.  First derivatives
-only.  Dropout masks are functions of (seed, offset, row, channel) and are recomputed in the backward pass."""
+in reverse mode only.  Dropout masks are functions of (seed, offset, row, channel) and are recomputed in the backward pass."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -64,7 +65,11 @@ class _DropoutAddLayerNormFn(torch.autograd.Function):
 
 
 def _taped(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    """Does autograd follow the call?  Dual tensors of forward-mode differentiation go the same way: the Functions have no
+    rule for tangents and say so, where the kernels alone would lose them."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

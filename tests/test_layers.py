@@ -271,3 +271,25 @@ def test_network_states_are_drawn_and_counted():
         net(dict(dropout_states=[None] * 3))
     with pytest.raises(ValueError, match="drops in 0 blocks"):
         spunet.SpUNet(**kw)(dict(dropout_states=[None]))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(definitions, monkeypatch, grad):
+    """Forward-mode differentiation has no rule here; the call says so, whichever argument carries the tangent, and a call
+    without tangents inside the same level runs."""
+    import torch.autograd.forward_ad as fw
+    for name in ("layer_norm_fwd", "dropout", "dropout_add_layer_norm_fwd"):   # raw addresses carry no tangent
+        fn = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, fn=fn: fn(*(t.detach() if isinstance(t, torch.Tensor) else t for t in a)))
+    x, w = torch.randn(4, 8), torch.ones(8)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        d, dw = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(w, torch.ones_like(w))
+        for call in (lambda: layers.layer_norm(d), lambda: layers.layer_norm(x, dw, w), lambda: layers.dropout(d, 0.5, seed=1),
+                     lambda: layers.dropout_add_layer_norm(d, x), lambda: layers.dropout_add_layer_norm(x, d, w, w),
+                     lambda: layers.dropout_add_layer_norm(x, x, w, dw)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        layers.layer_norm(x, w, w), layers.dropout_add_layer_norm(x, x, w, w, p=0.5, seed=1), layers.dropout(x, 0.5, seed=1)
+    assert torch.equal(layers.layer_norm(x, w, w), O.layer_norm(x.double(), w, w)[0].float())
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(layers.layer_norm, (x,), (x,))
