@@ -158,7 +158,8 @@ class Dropout(nn.Module):
 
 
 class DropoutAddLayerNorm(nn.Module):
-    """(x, residual) -> (y, h): h = residual + dropout(x), y = layer norm of h.  `state`: as in Dropout."""
+    """(x, residual) -> (y, h): h = residual + dropout(x), y = layer norm of h.  `state`: as in Dropout.  Whether values
+    are dropped goes by the mode of the `drop` module (`train()` and `eval()` set it with the block's own)."""
 
     def __init__(self, num_features, p=0.0, eps=1e-5, affine=True, seed=None):
         super().__init__()
@@ -167,4 +168,4 @@ class DropoutAddLayerNorm(nn.Module):
 
     def forward(self, x, residual, state=None):
         return dropout_add_layer_norm(x, residual, self.norm.weight, self.norm.bias, self.norm.eps, self.drop.p,
-                                      self.training, state=self.drop.draw() if state is None else state)
+                                      self.drop.training, state=self.drop.draw() if state is None else state)

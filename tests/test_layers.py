@@ -293,3 +293,22 @@ def test_tangents_are_refused(definitions, monkeypatch, grad):
     assert torch.equal(layers.layer_norm(x, w, w), O.layer_norm(x.double(), w, w)[0].float())
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.jvp(layers.layer_norm, (x,), (x,))
+
+
+def test_the_dropout_of_a_block_goes_by_its_own_mode(definitions):
+    """A block whose dropout alone was switched off drops nothing; one whose dropout alone is on draws a mask a call."""
+    calls = definitions
+    x = torch.randn(6, 8)
+    block = layers.DropoutAddLayerNorm(8, 0.5, seed=7)
+    block.drop.eval()
+    assert torch.equal(block(x, x)[1], 2 * x) and calls[-1] == (0.0, 0, 0, None)
+    assert torch.equal(block(x, x, ops.dropout_state(1, "cpu"))[1], 2 * x) and block.drop.rng.tolist() == [7, 0]
+    block.eval()
+    block.drop.train()
+    h0, h1 = block(x, x)[1], block(x, x)[1]
+    assert calls[-2:] == [(0.5, 0, 0, [7, 0]), (0.5, 0, 0, [7, 1])] and not torch.equal(h0, h1)
+    block.train()
+    block(x, x)
+    assert calls[-1] == (0.5, 0, 0, [7, 2])
+    block.eval()
+    assert torch.equal(block(x, x)[1], 2 * x) and block.drop.rng.tolist() == [7, 3]
