@@ -86,10 +86,10 @@ class PDLayerNorm(PDBatchNorm):
     pass each way (layers.dropout_add_layer_norm).  `eps` and `momentum` of the batch norms are not used."""
 
     def __init__(self, num_features, context_channels=256, conditions=CONDITIONS, decouple=True, adaptive=False,
-                 affine=True, dropout=0.0):
+                 affine=True, dropout=0.0, seed=None):
         super().__init__(num_features, context_channels, conditions=conditions, decouple=decouple, adaptive=adaptive,
                          affine=affine)
-        self.drop = layers.Dropout(dropout) if dropout > 0.0 else None
+        self.drop = layers.Dropout(dropout, seed) if dropout > 0.0 else None
 
     def forward(self, feat, condition=None, context=None, residual=None, relu=False, state=None):
         """`state`: what `drop.draw()` returned, for a call that is computed twice (activation checkpointing); None: the
@@ -234,9 +234,12 @@ class SpUNet(nn.Module):
     def __init__(self, in_channels=3, out_channels=768, num_classes=0, base_channels=32, context_channels=256,
                  channels=SPUNET34C["channels"], layers=SPUNET34C["layers"], conditions=CONDITIONS,
                  zero_init=True, norm_decouple=True, norm_adaptive=True, norm_affine=True,
-                 hash_method="fnv", pooling_method="mean", pooling_seed=0, norm="batch", dropout=0.0):
+                 hash_method="fnv", pooling_method="mean", pooling_seed=0, norm="batch", dropout=0.0,
+                 dropout_seed=None):
         """norm="layer": PDLayerNorm in place of PDBatchNorm, with `dropout` on the residual branch of every block while
-        training (runs and trains here; the fused engine takes batch norms only)."""
+        training (runs and trains here; the fused engine takes batch norms only).  dropout_seed: every block's generator
+        gets a seed of its own that follows from it; ranks that shall drop different values are given different ones.
+        None: the seeds are drawn from torch's generator."""
         super().__init__()
         if norm not in ("batch", "layer"):
             raise ValueError(f"unknown norm {norm!r} (batch or layer)")
@@ -253,8 +256,10 @@ class SpUNet(nn.Module):
         self.num_stages = len(layers) // 2
         self.conditions = tuple(conditions)
         self.zero_init = zero_init
+        seeds = None if dropout_seed is None else torch.Generator().manual_seed(dropout_seed)
+        block_seed = lambda: None if seeds is None else int(torch.randint(0, 2 ** 62, (), generator=seeds))
         make_norm = (lambda c: PDLayerNorm(c, context_channels, self.conditions, norm_decouple, norm_adaptive, norm_affine,
-                                           dropout)) if norm == "layer" else \
+                                           dropout, block_seed())) if norm == "layer" else \
                     (lambda c: PDBatchNorm(c, context_channels, 1e-3, 0.01, self.conditions, norm_decouple, norm_adaptive,
                                            norm_affine))
         ch = self.channels

@@ -312,3 +312,18 @@ def test_the_dropout_of_a_block_goes_by_its_own_mode(definitions):
     assert calls[-1] == (0.5, 0, 0, [7, 2])
     block.eval()
     assert torch.equal(block(x, x)[1], 2 * x) and block.drop.rng.tolist() == [7, 3]
+
+
+def test_dropout_seed_of_the_network():
+    """Networks of one dropout_seed drop alike, those of another differ in every block; blocks differ among themselves;
+    the seed leaves torch's generator and the parameters as they are."""
+    kw = dict(channels=(32, 64, 64, 32), layers=(1, 1, 1, 1), out_channels=32, norm="layer", dropout=0.1)
+    nets = []
+    for seed in (0, 0, 1, None):
+        torch.manual_seed(2)
+        nets.append(spunet.SpUNet(dropout_seed=seed, **kw))
+    seeds = [[m.rng[0].item() for m in net.modules() if isinstance(m, layers.Dropout)] for net in nets]
+    assert seeds[0] == seeds[1] and not set(seeds[0]) & set(seeds[2]) and not set(seeds[0]) & set(seeds[3])
+    assert all(len(set(s)) == len(s) for s in seeds)
+    assert all(m.rng[1] == 0 for m in nets[0].modules() if isinstance(m, layers.Dropout))
+    assert all(torch.equal(p, q) for p, q in zip(nets[0].parameters(), nets[2].parameters()))
