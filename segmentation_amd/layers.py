@@ -79,27 +79,43 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _LayerNormFn.apply(x, weight, bias, eps)
 
 
-def dropout(x, p=0.5, training=True, seed=0, offset=0, state=None):
-    """Dropout (ops.dropout), differentiable in x; x itself outside training or with p = 0.  Calls that shall draw
-    masks of their own differ in seed, offset or state (ops.dropout_next)."""
+def _mask_of(x, seed, offset, state):
+    """(seed, offset, state) of one call's mask: what was given, or a seed of its own from torch's CPU generator (which
+    activation checkpointing restores for the forward that it computes again)."""
+    if seed is None and offset is None and state is None:
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("dropout: a captured call needs a generator state (ops.dropout_next); a seed that is drawn "
+                               "on the host would be the same on every replay")
+        seed = int(torch.randint(0, 2 ** 62, (), device="cpu"))
+    return 0 if seed is None else seed, 0 if offset is None else offset, state
+
+
+def dropout(x, p=0.5, training=True, seed=None, offset=None, state=None):
+    """Dropout (ops.dropout), differentiable in x; x itself outside training or with p = 0.  The mask is a function of
+    (seed, offset) or of a `state` (ops.dropout_next); a call that is given none of them draws a seed from torch's
+    generator."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} is not in [0, 1]")
     if not training or p == 0.0:
         return x
+    seed, offset, state = _mask_of(x, seed, offset, state)
     if not _taped(x):
         return ops.dropout(x, p, seed, offset, state)
     return _DropoutFn.apply(x, p, seed, offset, state)
 
 
-def dropout_add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, training=True, seed=0, offset=0,
-                           state=None, need_h=True):
+def dropout_add_layer_norm(x, residual, weight=None, bias=None, eps=1e-5, p=0.0, training=True, seed=None,
+                           offset=None, state=None, need_h=True):
     """(y, h) with h = residual + dropout(x) and y = layer norm of h (ops.dropout_add_layer_norm_fwd), differentiable in
-    x, residual, weight and bias through both outputs; no dropout outside training.  The residual stream is of x's type or
-    float32.  need_h=False: the caller goes on with y alone (post-norm blocks); h is None where no gradient needs it."""
+    x, residual, weight and bias through both outputs; no dropout outside training; the mask as in `dropout`.  The
+    residual stream is of x's type or float32.  need_h=False: the caller goes on with y alone (post-norm blocks); h is None
+    where no gradient needs it."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} is not in [0, 1]")
     if not training or p == 0.0:
         p, seed, offset, state = 0.0, 0, 0, None
+    else:
+        seed, offset, state = _mask_of(x, seed, offset, state)
     if not _taped(x, residual, weight, bias):
         return ops.dropout_add_layer_norm_fwd(x, residual, weight, bias, eps, p, seed, offset, state, need_h)[:2]
     return _DropoutAddLayerNormFn.apply(x, residual, weight, bias, eps, p, seed, offset, state)

@@ -723,3 +723,24 @@ def test_checkpointed_backbone_with_dropout(device):
     rel = lambda a, b: float((a.double() - b.double()).norm() / b.double().norm())
     assert all(rel(a, b) < 1e-4 for a, b in zip(got, want))
     assert any(rel(a, b) > 1e-2 for a, b in zip(other, want))
+
+
+def test_a_captured_call_names_its_mask(device):
+    """Functions that would draw a seed on the host are refused under capture, and run outside."""
+    x = _randn(161, 8, 16).to(device)
+    torch.manual_seed(0)
+    a, b = layers.dropout(x, 0.5), layers.dropout(x, 0.5)
+    torch.manual_seed(0)
+    assert not torch.equal(a, b) and torch.equal(a, layers.dropout(x, 0.5))
+    st = ops.dropout_state(4, device)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="captured call"):
+            layers.dropout(x, 0.5)
+        with pytest.raises(RuntimeError, match="captured call"):
+            layers.dropout_add_layer_norm(x, x, p=0.5)
+        y = layers.dropout(x, 0.5, state=ops.dropout_next(st))
+    for k in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.dropout(x, 0.5, 4, k))

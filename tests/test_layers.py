@@ -327,3 +327,34 @@ def test_dropout_seed_of_the_network():
     assert all(len(set(s)) == len(s) for s in seeds)
     assert all(m.rng[1] == 0 for m in nets[0].modules() if isinstance(m, layers.Dropout))
     assert all(torch.equal(p, q) for p, q in zip(nets[0].parameters(), nets[2].parameters()))
+
+
+def test_functions_without_a_seed_draw_one(definitions):
+    """As torch's own dropout: two calls drop different values, torch's generator repeats them, and a recomputed forward
+    gets its first mask again.  What names a seed, an offset or a state has that mask."""
+    from torch.utils.checkpoint import checkpoint
+    calls = definitions
+    x = torch.randn(12, 16, requires_grad=True)
+    both = lambda t, **kw: (layers.dropout(t, 0.5, **kw), layers.dropout_add_layer_norm(t, t, p=0.5, **kw)[1])
+    torch.manual_seed(4)
+    a, b = both(x), both(x)
+    torch.manual_seed(4)
+    again = both(x)
+    for u, v, w in zip(a, b, again):
+        assert not torch.equal(u, v) and torch.equal(u, w)
+    for kw, seen in ((dict(seed=0), (0, 0, None)), (dict(offset=3), (0, 3, None)), (dict(offset=0), (0, 0, None)),
+                     (dict(seed=5, offset=6), (5, 6, None)), (dict(state=torch.tensor([8, 9])), (0, 0, [8, 9]))):
+        before = torch.get_rng_state()
+        both(x, **kw)
+        assert calls[-1] == calls[-2] == (0.5, *seen) and torch.equal(before, torch.get_rng_state())
+    before = torch.get_rng_state()
+    assert layers.dropout(x, 0.0) is x and layers.dropout(x, 0.5, False) is x
+    layers.dropout_add_layer_norm(x, x), layers.dropout_add_layer_norm(x, x, p=0.5, training=False)
+    assert torch.equal(before, torch.get_rng_state())
+    for reentrant in (False, True):
+        torch.manual_seed(5)
+        want = torch.autograd.grad(both(x)[0].square().sum(), x)[0]
+        torch.manual_seed(5)
+        x.grad = None
+        checkpoint(lambda t: both(t)[0], x, use_reentrant=reentrant).square().sum().backward()
+        assert torch.equal(x.grad, want) and want.abs().sum() > 0
