@@ -155,6 +155,13 @@ class Dropout(nn.Module):
             seed = int(torch.randint(0, 2 ** 62, ()))
         self.register_buffer("rng", ops.dropout_state(seed, "cpu"))
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        """A state dict without a generator (of nn.Dropout, or of a model that was trained without dropout) leaves the
+        module its own."""
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if prefix + "rng" in missing_keys:
+            missing_keys.remove(prefix + "rng")
+
     def draw(self):
         """The (seed, offset) of one call, or None where nothing is dropped."""
         if not (self.training and self.p > 0.0):

@@ -91,6 +91,12 @@ class PDLayerNorm(PDBatchNorm):
                          affine=affine)
         self.drop = layers.Dropout(dropout, seed) if dropout > 0.0 else None
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        """Without dropout the generator of a model that was trained with it is not needed."""
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if self.drop is None and prefix + "drop.rng" in unexpected_keys:
+            unexpected_keys.remove(prefix + "drop.rng")
+
     def forward(self, feat, condition=None, context=None, residual=None, relu=False, state=None):
         """`state`: what `drop.draw()` returned, for a call that is computed twice (activation checkpointing); None: the
         call draws its own."""

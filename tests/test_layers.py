@@ -358,3 +358,28 @@ def test_functions_without_a_seed_draw_one(definitions):
         x.grad = None
         checkpoint(lambda t: both(t)[0], x, use_reentrant=reentrant).square().sum().backward()
         assert torch.equal(x.grad, want) and want.abs().sum() > 0
+
+
+def test_state_dicts_with_and_without_generators():
+    """Strict loads both ways between a network with dropout and one without, a resumed generator, and a state dict of
+    nn.Dropout; other keys are as strict as before."""
+    kw = dict(channels=(32, 64, 64, 32), layers=(1, 1, 1, 1), out_channels=32, norm="layer")
+    with_drop, bare = spunet.SpUNet(dropout=0.1, dropout_seed=1, **kw), spunet.SpUNet(**kw)
+    twin = spunet.SpUNet(dropout=0.3, dropout_seed=2, **kw)
+    sd = with_drop.state_dict()
+    sd["enc.0.block0.bn2.drop.rng"][1] = 40
+    bare.load_state_dict(sd)
+    assert all(torch.equal(p, q) for p, q in zip(bare.parameters(), with_drop.parameters()))
+    seed = twin.enc[0].block0.bn2.drop.rng.clone()
+    twin.load_state_dict(bare.state_dict())
+    assert torch.equal(twin.enc[0].block0.bn2.drop.rng, seed)
+    twin.load_state_dict(sd)
+    assert twin.enc[0].block0.bn2.drop.rng.tolist() == sd["enc.0.block0.bn2.drop.rng"].tolist()
+    drop = layers.Dropout(0.2, seed=6)
+    drop.load_state_dict(torch.nn.Dropout(0.2).state_dict())
+    assert drop.rng.tolist() == [6, 0]
+    for bad in (dict(sd, extra=seed), {k: v for k, v in sd.items() if k != "enc.0.block0.bn2.bns.0.weight"},
+                {**sd, "enc.0.block0.bn2.drop.other": seed}):
+        for net in (twin, bare):
+            with pytest.raises(RuntimeError, match="key"):
+                net.load_state_dict(bad)
