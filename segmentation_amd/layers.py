@@ -152,8 +152,10 @@ class Dropout(nn.Module):
             raise ValueError(f"dropout probability {p} is not in [0, 1]")
         self.p = float(p)
         if seed is None:
-            seed = int(torch.randint(0, 2 ** 62, ()))
-        self.register_buffer("rng", ops.dropout_state(seed, "cpu"))
+            seed = int(torch.randint(0, 2 ** 62, (), device="cpu"))
+        # where a module's buffers are made; a generator has a value from the start, also in a module without storage
+        device = torch.get_default_device()
+        self.register_buffer("rng", ops.dropout_state(seed, "cpu" if device.type == "meta" else device))
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         """A state dict without a generator (of nn.Dropout, or of a model that was trained without dropout) leaves the

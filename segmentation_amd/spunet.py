@@ -262,8 +262,8 @@ class SpUNet(nn.Module):
         self.num_stages = len(layers) // 2
         self.conditions = tuple(conditions)
         self.zero_init = zero_init
-        seeds = None if dropout_seed is None else torch.Generator().manual_seed(dropout_seed)
-        block_seed = lambda: None if seeds is None else int(torch.randint(0, 2 ** 62, (), generator=seeds))
+        seeds = None if dropout_seed is None else torch.Generator(device="cpu").manual_seed(dropout_seed)
+        block_seed = lambda: None if seeds is None else int(torch.randint(0, 2 ** 62, (), generator=seeds, device="cpu"))
         make_norm = (lambda c: PDLayerNorm(c, context_channels, self.conditions, norm_decouple, norm_adaptive, norm_affine,
                                            dropout, block_seed())) if norm == "layer" else \
                     (lambda c: PDBatchNorm(c, context_channels, 1e-3, 0.01, self.conditions, norm_decouple, norm_adaptive,

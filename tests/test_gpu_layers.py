@@ -744,3 +744,14 @@ def test_a_captured_call_names_its_mask(device):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ops.dropout(x, 0.5, 4, k))
+
+
+def test_modules_made_on_the_device(device):
+    """Under a default device the generator lies where the parameters do."""
+    with torch.device(device):
+        block = layers.DropoutAddLayerNorm(16, 0.5, seed=2)
+        drawn = layers.Dropout(0.5)
+    assert block.drop.rng.device == block.norm.weight.device == drawn.rng.device
+    x = _randn(171, 4, 16).to(device)
+    assert torch.equal(block(x, x)[1], ops.dropout_add_layer_norm_fwd(x, x, p=0.5, seed=2)[1])
+    assert drawn(x).shape == x.shape

@@ -383,3 +383,19 @@ def test_state_dicts_with_and_without_generators():
         for net in (twin, bare):
             with pytest.raises(RuntimeError, match="key"):
                 net.load_state_dict(bad)
+
+
+def test_modules_under_a_default_device():
+    """Constructed without storage (to be filled by load_state_dict(assign=True)), a module still has a generator."""
+    with torch.device("meta"):
+        block = layers.DropoutAddLayerNorm(8, 0.5)
+        seeded = layers.Dropout(0.5, seed=12)
+    assert block.norm.weight.is_meta and block.drop.rng.device.type == "cpu" and seeded.rng.tolist() == [12, 0]
+    source = layers.DropoutAddLayerNorm(8, 0.5, seed=3)
+    block.load_state_dict(source.state_dict(), assign=True)
+    assert not block.norm.weight.is_meta and block.drop.rng.tolist() == [3, 0]
+    kw = dict(channels=(32, 64, 64, 32), layers=(1, 1, 1, 1), out_channels=32, norm="layer", dropout=0.1, dropout_seed=3)
+    here = spunet.SpUNet(**kw)
+    with torch.device("meta"):
+        there = spunet.SpUNet(**kw)
+    assert torch.equal(there.enc[0].block0.bn2.drop.rng, here.enc[0].block0.bn2.drop.rng)
