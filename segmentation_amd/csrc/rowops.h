@@ -103,26 +103,39 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __builtin_bit_cast(float, o);
 }
 
-// Sum over aligned groups of g lanes (g a power of two, 1..64, the same in every lane); every lane gets it.  The
-// four steps inside 16 lanes are lane permutations of the add itself, 16 and 32 are row and half swaps.
-__device__ __forceinline__ float group_sum(float v, int g) {
-  if (g > 1) v = dpp_add<0xB1>(v);    // lane ^ 1
-  if (g > 2) v = dpp_add<0x4E>(v);    // lane ^ 2
-  if (g > 4) v = dpp_add<0x141>(v);   // mirror inside 8 lanes (quads are equal by now)
-  if (g > 8) v = dpp_add<0x140>(v);   // mirror inside 16 lanes
-  if (g > 16) {
-    const int b = __builtin_bit_cast(int, v);
-    const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-    const unsigned lo = s[0], hi = s[1];
-    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-  }
-  if (g > 32) {
-    const int b = __builtin_bit_cast(int, v);
-    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    const unsigned lo = s[0], hi = s[1];
-    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-  }
-  return v;
+// Sums over aligned groups of g lanes (g a power of two, 1..64, the same in every lane); every lane gets them.  The
+// four steps inside 16 lanes are lane permutations of the add itself, 16 and 32 are row and half swaps.  The sums go
+// through a step together, so that two take little longer than one.
+template <int NQ>
+__device__ __forceinline__ void group_sum(float (&v)[NQ], int g) {
+  if (g > 1)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) v[q] = dpp_add<0xB1>(v[q]);    // lane ^ 1
+  if (g > 2)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) v[q] = dpp_add<0x4E>(v[q]);    // lane ^ 2
+  if (g > 4)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) v[q] = dpp_add<0x141>(v[q]);   // mirror inside 8 lanes (quads are equal by now)
+  if (g > 8)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) v[q] = dpp_add<0x140>(v[q]);   // mirror inside 16 lanes
+  if (g > 16)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int b = __builtin_bit_cast(int, v[q]);
+      const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+      const unsigned lo = s[0], hi = s[1];
+      v[q] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    }
+  if (g > 32)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int b = __builtin_bit_cast(int, v[q]);
+      const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+      const unsigned lo = s[0], hi = s[1];
+      v[q] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    }
 }
 
 // ---------------------------------------------------------------- dropout masks

@@ -755,3 +755,48 @@ def test_modules_made_on_the_device(device):
     x = _randn(171, 4, 16).to(device)
     assert torch.equal(block(x, x)[1], ops.dropout_add_layer_norm_fwd(x, x, p=0.5, seed=2)[1])
     assert drawn(x).shape == x.shape
+
+
+@pytest.mark.parametrize("xt", [F32, BF16])
+@pytest.mark.parametrize("n,c", [(5, 3), (4, 7), (9, 33), (6, 96), (7, 100), (5, 768), (3, 1001), (2, 5000), (2, 16383)])
+def test_rows_far_from_zero(device, n, c, xt):
+    """Rows whose values lie far from zero against their deviations (equal values among them): y must not depend on where
+    they lie.  The first mean m is off by at most d = D u A; the deviations from it are exact up to u of themselves (they
+    are small against the values), so with E the row's mean of |x - mean| the corrected mean is off by D u (E + d).  The
+    variance is off by (D + 8) u (var + 2 d^2), of which rstd has half relative to var + eps."""
+    for scale, shift in ((0.0, 1234.567), (0.0, -77.7), (0.0, 98765.4), (1.0, 1000.3), (0.1, -1e4), (1.0, 1e5)):
+        x = _randn(181, n, c, scale=scale, shift=shift).to(xt)
+        X = x.double()
+        w, b = _randn(182, c, shift=1.0), _randn(183, c)
+        W, B = w.double(), b.double()
+        Y, MEAN, RSTD = O.layer_norm(X, W, B)
+        d = D * U * X.abs().mean(1)
+        e = (X - MEAN[:, None]).abs().mean(1)
+        rel = (D + 8) * U * (1 / RSTD ** 2 + 2 * d ** 2) * RSTD ** 2
+        hat = (X - MEAN[:, None]) * RSTD[:, None]
+        eh = RSTD[:, None] * (D * U * (e + d))[:, None] + (rel[:, None] + 10 * U) * hat.abs()
+        ty = 2 * (W.abs() * eh + 4 * U * ((W * hat).abs() + B.abs()))
+        wg, bg = w.to(device), b.to(device)
+        if xt == F32:
+            y, mean, rstd = ops.layer_norm_fwd(x.to(device), wg, bg)
+            _close("y", y, Y, ty + _half(F32, Y.abs() + ty))
+        else:   # behind the add, whose stream is f32: 16-bit rows lie too far apart to be told from their mean
+            zero = torch.zeros(n, c, dtype=xt, device=device)
+            y, _, mean, rstd = ops.dropout_add_layer_norm_fwd(zero, x.float().to(device), wg, bg)
+            _close("y", y, Y, ty + _half(xt, Y.abs() + ty))
+        _close("mean", mean, MEAN, U * MEAN.abs() + 2 * D * U * (e + d))   # one rounding of the mean itself
+        _close("rstd", rstd, RSTD, 2 * rel * RSTD)
+        if scale == 0.0:
+            assert torch.equal(mean.cpu(), x[:, 0].float())
+            dy = _randn(184, n, c, dtype=xt).to(device)
+            back = ops.layer_norm_backward(x.to(device), dy, mean, rstd, wg)
+            assert (back[1] == 0).all()
+
+
+def test_overflowing_squares_leave_the_bias(device):
+    """Values whose squares leave float32: rstd is 0 and y the bias, also where all values are equal."""
+    b = _randn(191, 33).to(device)
+    for x in (torch.full((3, 33), 1e36), _randn(192, 3, 33, scale=1e25)):
+        y, _, rstd = ops.layer_norm_fwd(x.to(device), None, b)
+        assert torch.isfinite(y).all()
+    assert torch.equal(y, b.expand(3, 33)) and (rstd == 0).all()
