@@ -800,3 +800,128 @@ def test_overflowing_squares_leave_the_bias(device):
         y, _, rstd = ops.layer_norm_fwd(x.to(device), None, b)
         assert torch.isfinite(y).all()
     assert torch.equal(y, b.expand(3, 33)) and (rstd == 0).all()
+
+
+# ---------------------------------------------------------------- more rows than one sweep of the launch covers
+@pytest.mark.parametrize("n,c,xt,rt,wt", [
+    (40011, 96, F32, F32, F32), (40001, 64, BF16, F32, F32), (70001, 33, F32, F32, F32), (17001, 333, F16, F16, F16),
+    (70003, 77, BF16, BF16, F32),                                  # f32 weights on a 16-bit stream
+    (1101, 4096, BF16, BF16, BF16), (601, 3000, F32, F32, F32),    # rows of 256 lanes: workgroups of 512 in the backward pass
+    (701, 7000, BF16, F32, F32),                                   # rows of 512 lanes
+    (300, 9000, F32, F32, F32), (301, 13001, BF16, BF16, F32)])    # rows of 1024 lanes
+def test_add_over_several_tiles(device, n, c, xt, rt, wt):
+    """Every workgroup walks over several tiles: the next tile's rows, the mask's row index, dh beside the tile in flight
+    and the column sums over all of them.  p = 0.5 doubles exactly, so h is known to the bit."""
+    p, seed, offset = 0.5, 77, 5
+    x, r = _randn(201, n, c, dtype=xt, scale=1.5), _randn(202, n, c, dtype=rt, scale=2.0, shift=0.3)
+    dy, dh = _randn(203, n, c, dtype=xt), _randn(204, n, c, dtype=rt)
+    w, b = _randn(205, c, dtype=wt, scale=0.2, shift=1.0), _randn(206, c, dtype=wt, scale=0.3)
+    keep = O.dropout_keep(n, c, p, seed, offset)
+    H = (r.float() + torch.where(keep, x.float() * 2, torch.zeros(()))).to(rt)
+    HD, DY, W, B = H.double(), dy.double(), w.double(), b.double()
+    Y, MEAN, RSTD = O.layer_norm(HD, W, B)
+    DX, DW, DB = O.layer_norm_backward(HD, DY, MEAN, RSTD, W)
+    kw = dict(p=p, seed=seed, offset=offset)
+    wg, dyg = w.to(device), dy.to(device)
+    y, h, mean, rstd = ops.dropout_add_layer_norm_fwd(x.to(device), r.to(device), wg, b.to(device), **kw)
+    assert torch.equal(h.cpu(), H)
+    ty = _tol_y(HD, W, B, MEAN, RSTD)
+    _close("y", y, Y, ty + _half(xt, Y.abs() + ty))
+    T = DX + dh.double()
+    tt = _tol_dx(HD, DY, W, MEAN, RSTD, DX) + U * T.abs()
+    dx, dr, dw, db = ops.dropout_add_layer_norm_backward(h, dyg, dh.to(device), mean, rstd, wg, **kw)
+    _close("dresidual", dr, T, tt + _half(rt, T.abs() + tt))
+    TX, tx = 2 * T, 2 * tt + 4 * U * T.abs()
+    zero = torch.zeros((), dtype=torch.float64)
+    _close("dx", dx, torch.where(keep, TX, zero), torch.where(keep, tx + _half(xt, TX.abs() + tx), zero))
+    tw, tb = _tol_columns(HD, DY, MEAN, RSTD)
+    _close("dw", dw, DW, tw + _half(wt, DW.abs() + tw))
+    _close("db", db, DB, tb + _half(wt, DB.abs() + tb))
+    if xt == rt:   # the norm alone over as many tiles
+        dx, dw, db = ops.layer_norm_backward(h, dyg, mean, rstd, wg)
+        tx = _tol_dx(HD, DY, W, MEAN, RSTD, DX)
+        _close("dx alone", dx, DX, tx + _half(xt, DX.abs() + tx))
+        _close("dw alone", dw, DW, tw + _half(wt, DW.abs() + tw))
+        _close("db alone", db, DB, tb + _half(wt, DB.abs() + tb))
+
+
+def test_captured_graphs_have_workspaces_of_their_own(device, monkeypatch):
+    """Two backward passes captured on one stream, of different inputs: their workspaces differ from each other and from
+    every eager one, and replayed side by side on two streams, beside eager work, each gives its own result."""
+    n, c = 4000, 512
+    ins = [(_randn(211 + k, n, c).to(device), _randn(213 + k, n, c).to(device)) for k in range(2)]
+    stats = [ops.layer_norm_fwd(x)[1:] for x, _ in ins]
+    want = [ops.layer_norm_backward(x, dy, *st) for (x, dy), st in zip(ins, stats)]
+    torch.cuda.synchronize()
+    real, spans, graphs = ops._scratch, [], []
+
+    def recorded(nbytes, dev):
+        ws = real(nbytes, dev)
+        spans.append((ws.data_ptr(), ws.data_ptr() + ws.numel()))
+        return ws
+
+    side = torch.cuda.Stream()
+    monkeypatch.setattr(ops, "_scratch", recorded)
+    for (x, dy), st in zip(ins, stats):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = ops.layer_norm_backward(x, dy, *st)
+        graphs.append((g, out))
+    monkeypatch.setattr(ops, "_scratch", real)
+    assert len(spans) == 2
+    spans += [(t.data_ptr(), t.data_ptr() + t.numel()) for t in ops._workspaces.values()]
+    spans.sort()
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), spans
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(side):
+            ops.layer_norm_backward(*ins[1], *stats[1])
+        torch.cuda.synchronize()
+        for (_, out), ref in zip(graphs, want):
+            assert all(torch.equal(a, e) for a, e in zip(out, ref))
+            for t in out:
+                t.zero_()
+
+
+@pytest.mark.parametrize("decouple,adaptive,affine", [(True, True, True), (True, True, False), (False, False, True)])
+@pytest.mark.parametrize("given", [False, True])
+def test_pd_layer_norm_with_dropout_matches_float64(device, decouple, adaptive, affine, given):
+    """A training block: relu(layer norm(residual + dropout(x)) (1 + scale) + shift) and its gradients, with the mask of the
+    module's generator, drawn by the call or handed in.  Bars as in test_pd_layer_norm_matches_float64."""
+    torch.manual_seed(12)
+    p, n, c = 0.5, 90, 48
+    m = spunet.PDLayerNorm(c, 32, decouple=decouple, adaptive=adaptive, affine=affine, dropout=p, seed=21)
+    for q in m.parameters():
+        q.data.normal_(0.0, 0.3)
+    ref = copy.deepcopy(m).double()
+    m = m.to(device)
+    x, res, ctx, gy = _randn(221, n, c), _randn(222, n, c), _randn(223, 1, 32), _randn(224, n, c)
+    for call in range(2):
+        ins = [t.to(device).requires_grad_() for t in (x, res, ctx)]
+        X, R, C = (t.double().requires_grad_() for t in (x, res, ctx))
+        m.zero_grad(), ref.zero_grad()
+        y = m(ins[0], "Matterport3D", ins[2], residual=ins[1], relu=True, **(dict(state=m.drop.draw()) if given else {}))
+        assert m.drop.rng.tolist() == [21, call + 1]
+        H = R + torch.where(O.dropout_keep(n, c, p, 21, call), X * 2, torch.zeros((), dtype=torch.float64))
+        D = H - H.mean(1, keepdim=True)
+        Y = D * (D.square().mean(1, keepdim=True) + 1e-5).rsqrt()
+        ln = ref.bns[2] if decouple else ref.bn
+        if affine:
+            Y = Y * ln.weight + ln.bias
+        if adaptive:
+            shift, scale = ref.modulation(C).chunk(2, dim=1)
+            Y = Y * (1.0 + scale) + shift
+        g = gy * (Y.detach().abs() > 1e-4).float()   # no gradient within rounding distance of the kink
+        Y = Y.clamp_min(0)
+        y.backward(g.to(device))
+        Y.backward(g.double())
+        rel = lambda a, e: float((a.detach().double().cpu() - e).norm() / e.norm())
+        assert rel(y, Y.detach()) < 1e-5 and rel(ins[0].grad, X.grad) < 1e-5 and rel(ins[1].grad, R.grad) < 1e-5
+        assert not adaptive or rel(ins[2].grad, C.grad) < 1e-4
+        for (k, q), (_, e) in zip(m.named_parameters(), ref.named_parameters()):
+            assert (q.grad is None) == (e.grad is None), k
+            assert e.grad is None or rel(q.grad, e.grad) < 1e-4, k
