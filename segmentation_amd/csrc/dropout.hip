@@ -10,7 +10,7 @@ constexpr int kDropThreads = 256;
 // the row), the division by the pieces of a row is a multiplication (magic, shift: exact below 2^31 pieces).  WHOLE: no row
 // ends inside a piece.
 // Bound by HBM: the generator's 7 rounds are 14 widening products for 4 values, which the memory time covers (273080 x 96
-// f32 34.0 us, 6.2 TB/s; 16384 x 4096 bf16 45.2 us, 5.9 TB/s).
+// f32 34.2 us, 6.1 TB/s; 16384 x 4096 bf16 44.9 us, 6.0 TB/s).
 template <typename T, int U, bool WHOLE>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* __restrict__ x, int64_t ldx, int c, int64_t row0,
                                                                uint32_t total, uint32_t per_row, uint32_t magic,
@@ -71,9 +71,9 @@ static int dropout_launch(const T* x, int64_t ldx, int64_t n, int c, const DropA
   return M3D_OK;
 }
 
-// Pieces a thread: two of whole 16-bit pieces (16384 x 4096 bf16: 47.5 us, with one 52.0, with four 47.2), one otherwise
-// (273080 x 96 f32: 35.2 us, with two 36.2, with four 39.9; 75401 x 333 f16, whose rows end inside a piece: 22.6, with
-// two 25.2).
+// Pieces a thread: two of whole 16-bit pieces (16384 x 4096 bf16, the call on x and on the gradient: 93.8 us, with one
+// 94.6), one otherwise (273080 x 96 f32: 34.2 us, with two 34.9, with four 34.4; 75401 x 333 f16, whose rows end inside a
+// piece: 23.2, with two 25.4, with four 26.5).
 template <typename T>
 static int dropout_typed(const void* x, int64_t ldx, int64_t n, int c, const DropArgs& d, void* y, hipStream_t stream) {
   const T* from = static_cast<const T*>(x);

@@ -14,9 +14,10 @@
 // one partial row per workgroup and added up by a second launch in a fixed order (no atomics: run-to-run identical).
 //
 // Bound by HBM: 2 values moved for each forward, 3 for each backward (4 and 5 with the add), about 20 operations a value.
-// Kernel times, with 2 x FETCH_SIZE + WRITE_SIZE within 2 % of those bytes: 273080 x 96 f32 35.7 us forward (5.9 TB/s),
-// 54.2 backward (5.8); 75401 x 768 bf16 39.9 and 59.8 (5.8); 16384 x 4096 bf16 with dropout and add 99.5 (5.4) and 124.3
-// (5.4); the join of the columns 4.8.  A copy of 1 GB runs at 5.2.
+// Kernel times, with 2 x FETCH_SIZE + WRITE_SIZE within 2 % of those bytes: 273080 x 96 f32 35.9 us forward (5.8 TB/s),
+// 53.9 backward (5.8); 75401 x 768 bf16 39.8 and 59.0 (5.8, 5.9); 16384 x 4096 bf16 with dropout and add 102.8 (5.2) and
+// 123.9 (5.4); the join of the columns 4.7.  A copy of 1 GB runs at 5.2.  Where a workgroup gets few rows the partial rows
+// weigh more: 3493 x 1001 f16 backward moves 32 % above its 21 MB in the first launch, and 6 MB again in the join.
 #include "rowops.h"
 
 namespace m3d {
@@ -126,8 +127,10 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
   return a * b;
 }
 
+// Alone, the norm is held to the 128 registers at which the chip holds the workgroups that ln_blocks starts (65 bf16
+// channels 4.0 TB/s, with the 129 that it would take 3.2).  With the add some rows need more and would spill.
 template <typename TX, typename TR, int K, bool ADD, bool RAGGED, int THREADS>
-__global__ __launch_bounds__(THREADS) void ln_fwd_kernel(LnArgs a) {
+__global__ __launch_bounds__(THREADS, ADD ? 1 : 4) void ln_fwd_kernel(LnArgs a) {
   constexpr int V = kPiece<TX>;
   __shared__ float red[2][THREADS / 64][2];
   RowSum<THREADS> row_sum{red};
@@ -181,8 +184,8 @@ __global__ __launch_bounds__(THREADS) void ln_fwd_kernel(LnArgs a) {
     // The mean is off by the rounding of its sum, a few steps of the row's magnitude, which may be as large as sqrt(eps) or
     // as the deviations themselves (96 equal values between 1000 and 2000 gave |y| up to 0.15).  The deviations are exact
     // there, so their own mean is added back to it and taken out of them and, squared, of the variance.  The second sum
-    // costs nothing where the memory binds (273080 x 96 f32 forward and backward 93.2 us with and without), most on rows of
-    // eight waves (8192 x 8192 bf16 47.7 us, without 45.2).
+    // costs nothing where the memory binds (forward and backward of 273080 x 96 f32 101 us, 8192 x 8192 bf16 forward 44.4
+    // us, with and without); rows of sixteen waves wait for it (16384 bf16 channels 4.8 TB/s, without 5.2; f32 6.2, 6.3).
     const float about = rounded_product(s[0], a.inv_c);
     float dev[2] = {0.f, 0.f};
 #pragma unroll
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(1024) void ln_columns_kernel(const float* __restric
 
 // ---------------------------------------------------------------- launch shapes
 constexpr int kLnMaxChannels = 16384;
-constexpr int kLnMaxStride = 1 << 20;  // elements: a tile's rows (1024 at most) stay within 32-bit offsets
+constexpr int kLnMaxStride = 1 << 20;  // elements: a tile's rows (256 at most) stay within 32-bit offsets
 
 struct LnShape {
   int lg, k, threads;
@@ -452,7 +455,8 @@ static LnShape ln_shape(int c, int type) {
 //              8192 bf16 channels 56 against 47.6 us, with four times as many 59)
 //   backward:  512 threads a CU, or 768 where a lane has 64 bytes in flight or fewer (500000 x 32 f32: 39 against 44 us;
 //              75401 x 768 bf16, 96 bytes: 71 with 512 against 83 with 768, which no longer fit the registers at once).
-//              Rows of a group of 256 lanes take workgroups of 512, two rows at a time: half the partial rows.
+//              Rows of a group of 256 lanes take workgroups of 512, two rows at a time: half the partial rows.  Rows
+//              of 1024 lanes are a workgroup each, 1024 threads a CU.
 constexpr int kLnCus = 256;
 static LnShape ln_bwd_shape(int c, int type) {
   LnShape s = ln_shape(c, type);
