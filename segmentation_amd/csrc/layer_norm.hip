@@ -182,7 +182,7 @@ __global__ __launch_bounds__(THREADS, ADD ? 1 : 4) void ln_fwd_kernel(LnArgs a) 
     if (tile + gridDim.x < a.tiles) fetch(tile + gridDim.x);
     row_sum(s, a.lg);
     // The mean is off by the rounding of its sum, a few steps of the row's magnitude, which may be as large as sqrt(eps) or
-    // as the deviations themselves (96 equal values between 1000 and 2000 gave |y| up to 0.15).  The deviations are exact
+    // as the deviations themselves (96 equal values between 1000 and 2000 gave |y| up to 0.12).  The deviations are exact
     // there, so their own mean is added back to it and taken out of them and, squared, of the variance.  The second sum
     // costs nothing where the memory binds (forward and backward of 273080 x 96 f32 101 us, 8192 x 8192 bf16 forward 44.4
     // us, with and without); rows of sixteen waves wait for it (16384 bf16 channels 4.8 TB/s, without 5.2; f32 6.2, 6.3).

@@ -82,8 +82,9 @@ class PDBatchNorm(nn.Module):
 class PDLayerNorm(PDBatchNorm):
     """PDBatchNorm with layer norms (the norms that Point Prompt Training pairs with transformer blocks): the same
     per-dataset affine pairs under the same parameter names, the same context modulation, no running statistics.  A
-    residual is added in FRONT of the norm, as in a post-norm block: y = relu?(layer norm(residual + dropout(x))), one
-    pass each way (layers.dropout_add_layer_norm).  `eps` and `momentum` of the batch norms are not used."""
+    residual is added in FRONT of the norm, as in a post-norm block: y = relu?(layer norm(residual + dropout(x))).
+    Dropout, add and norm are one pass each way (layers.dropout_add_layer_norm), the ReLU is one of its own.  `eps` and
+    `momentum` of the batch norms are not used."""
 
     def __init__(self, num_features, context_channels=256, conditions=CONDITIONS, decouple=True, adaptive=False,
                  affine=True, dropout=0.0, seed=None):
